@@ -361,6 +361,79 @@ void ntcb_p2p_release(ntcb_trainer* t);
 void ntcb_p2p_set_poll_limit(ntcb_trainer* t, unsigned polls);
 int ntcb_p2p_barrier(ntcb_trainer* t, unsigned polls);
 
+/* ---- operators for learned models of the symbols (additions; no counterpart in the reference, which rates its symbols
+ * by counts and knows one Adam). They work on the caller's DEVICE buffers, on `stream` (a cudaStream_t; NULL = the
+ * legacy default stream) of `device` (-1 = the current one, which is left current), without synchronising and without
+ * allocating; the caller keeps the buffers alive until the stream is through. They never end the process: 1 on
+ * success, 0 with a reason in why otherwise, nothing launched. A CUDA error pending before the call is a refusal. All of
+ * them can be captured into a CUDA graph. Buffers that a call writes must not overlap any other of its buffers, except
+ * where that is allowed below. */
+enum { NTCB_F32 = 0, NTCB_F16 = 1, NTCB_BF16 = 2 };
+enum { NTCB_SYM_U8 = 0, NTCB_SYM_I16 = 1, NTCB_SYM_I32 = 2, NTCB_SYM_I64 = 3 };
+#define NTCB_MAX_TOPK 32
+/* Symbols under a predictor: `rows` rows of `vocab` logits (row r at logits + r * row_stride elements, its logits
+ * contiguous; row_stride 0 repeats one row) and one symbol per row (at symbols + r * symbol_stride). Strides in elements. */
+typedef struct ntcb_symbol_desc {
+    int device;
+    int dtype;            /* NTCB_F32 / F16 / BF16 */
+    int symbol_type;      /* NTCB_SYM_* */
+    int reserved;         /* 0 */
+    long long rows, vocab, row_stride, symbol_stride;
+} ntcb_symbol_desc;
+/* logp[r] = log p(symbol r), entropy[r] and lse[r] (log of the sum of exponentials) in nats, computed in 32 bits; and,
+ * for topk > 0 (at most NTCB_MAX_TOPK and vocab), the topk likeliest symbols of each row, likeliest first and the lower
+ * index first among equals: top_ids / top_logp [rows][topk]. A code length in bits is -logp / ln 2.
+ * A negative symbol is none: logp 0. A symbol >= vocab: logp NaN. A row whose logits are all -inf: lse and logp -inf,
+ * entropy 0. Logits of -inf are no alternatives: the places left over hold -1 and -inf. A row with a NaN or +inf
+ * logit: NaN, with ids -1. */
+int ntcb_symbol_logprobs(const ntcb_symbol_desc* d, const void* logits, const void* symbols, int topk, float* logp, float* entropy,
+                         float* lse, int* top_ids, float* top_logp, void* stream, char* why, size_t why_cap);
+/* The gradient of sum_r dlogp[r] logp[r] + dentropy[r] entropy[r] for the logits, in the logits' type. lse and entropy
+ * are the forward pass's (entropy is read only with dentropy, which may be NULL). The strides of dlogp and dentropy
+ * may be 0 (one value for every row). dlogits may be the logits' own buffer with their stride. Rows without a finite
+ * logit and, for the logp part, rows without a symbol get 0; rows the forward pass gave NaN get NaN. */
+int ntcb_symbol_logprobs_grad(const ntcb_symbol_desc* d, const void* logits, const void* symbols, const float* lse, const float* entropy,
+                              const float* dlogp, long long dlogp_stride, const float* dentropy, long long dentropy_stride, void* dlogits,
+                              long long dlogits_stride, void* stream, char* why, size_t why_cap);
+
+/* AdamW over many tensors in one step: m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2 (g the gradient times
+ * grad_scale), p = (1 - lr weight_decay) p - lr (m / (1 - b1^it)) / (sqrt(v / (1 - b2^it)) + eps), in 32 bits, the
+ * parameters rounded to nearest where they are held in 16. With weight_decay 0 it is the trainer's own Adam.
+ * A plan holds the tensors' sizes and types and a device table of the work, no pointer of the caller's; the moments are
+ * the caller's buffer of ntcb_adamw_state_bytes bytes (256-byte aligned, zeroed before the first step).
+ *
+ * The moments lie flat: tensor i at element ntcb_adamw_offset(i) (a multiple of 256), `total` = offset(ntensors)
+ * elements in all. state_bits 32: m [total] floats, then v [total] floats. state_bits 8: m codes [total] bytes, v codes
+ * [total] bytes, then a 16-bit window per 256 elements for m, then for v. A code stands for a float's exponent and
+ * upper 3 mantissa bits, q = bits >> 20, counted from the window's base: q = base + code, 0 is zero; m has 7 bits (126
+ * steps below the block's largest) and a sign, v 8 (254 steps); the highest code is NaN. Rounding is stochastic (unbiased
+ * down to the window's end), by the library's counter noise keyed on (seed, it, tensor, element): the same step gives
+ * the same bits. A v above zero never rounds to zero. */
+typedef struct ntcb_adamw ntcb_adamw;
+typedef struct ntcb_adamw_args {
+    double lr, beta1, beta2, eps, weight_decay, grad_scale;
+    long long it;                  /* step number, from 1, below 2^32 */
+    uint64_t seed;                 /* of the 8-bit rounding */
+    /* DEVICE scalars, NULL for the values above; a step captured into a graph must take `it` from the device. */
+    const long long* it_dev;
+    const float* lr_dev;
+    const float* grad_scale_dev;   /* multiplies grad_scale */
+} ntcb_adamw_args;
+/* Makes a plan for ntensors tensors of sizes[i] elements (0 allowed) of param_types[i] with gradients of grad_types[i].
+ * Allocates the device table: not during a stream capture. NULL with a reason on failure. */
+ntcb_adamw* ntcb_adamw_create(int device, int ntensors, const long long* sizes, const int* param_types, const int* grad_types,
+                              int state_bits, char* why, size_t why_cap);
+void ntcb_adamw_destroy(ntcb_adamw* a);
+size_t ntcb_adamw_state_bytes(const ntcb_adamw* a);
+long long ntcb_adamw_offset(const ntcb_adamw* a, int tensor);   /* tensor == ntensors: total; -1 out of range */
+/* One step. params[i] / grads[i]: HOST arrays of device pointers; a NULL gradient leaves its tensor and moments as they are. */
+int ntcb_adamw_step(const ntcb_adamw* a, void* const* params, const void* const* grads, void* state, const ntcb_adamw_args* args,
+                    void* stream, char* why, size_t why_cap);
+/* The moments as floats, m [total] and v [total] (elements between tensors are 0); and back, rounded to nearest where
+ * the state has 8 bits. */
+int ntcb_adamw_get_moments(const ntcb_adamw* a, const void* state, float* m, float* v, void* stream, char* why, size_t why_cap);
+int ntcb_adamw_set_moments(const ntcb_adamw* a, const float* m, const float* v, void* state, void* stream, char* why, size_t why_cap);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,7 +3,8 @@ neural_block_textures, behind the reference's ntc_cuda::Trainer interface.
 
 The product is libntc_b200.so (CUDA kernels + host engine + C ABI + the C++ class). This package
 builds it (build.py), binds it (abi.py, trainer.py) and describes models and benchmark
-configurations (model.py, synth.py, dct.py).
+configurations (model.py, synth.py, dct.py). The operators on the caller's own device tensors (symbols.py:
+log probabilities of symbols and their gradient; optim.py: AdamW) take torch tensors and load torch on first use.
 """
 from .abi import DctDesc, ModelDesc, QesDesc, load_library
 from .model import CONFIGS, LevelSpec, ModelSpec, TrainConfig, config, qat_grid_table
@@ -11,3 +12,13 @@ from .trainer import Trainer
 
 __all__ = ["Trainer", "ModelDesc", "QesDesc", "DctDesc", "load_library", "ModelSpec", "LevelSpec", "TrainConfig",
            "CONFIGS", "config", "qat_grid_table"]
+
+_TORCH_NAMES = {"symbol_logprobs": "symbols", "symbol_logprobs_grad": "symbols", "SymbolLogprobs": "symbols", "AdamW": "optim"}
+__all__ += list(_TORCH_NAMES)
+
+
+def __getattr__(name):
+    if name in _TORCH_NAMES:
+        from importlib import import_module
+        return getattr(import_module("." + _TORCH_NAMES[name], __name__), name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -101,6 +101,23 @@ class ProgressStats(C.Structure):
     ]
 
 
+class SymbolDesc(C.Structure):
+    """ntcb_symbol_desc: rows of logits and the symbols they rate."""
+    _fields_ = [
+        ("device", C.c_int), ("dtype", C.c_int), ("symbol_type", C.c_int), ("reserved", C.c_int),
+        ("rows", C.c_longlong), ("vocab", C.c_longlong), ("row_stride", C.c_longlong), ("symbol_stride", C.c_longlong),
+    ]
+
+
+class AdamWArgs(C.Structure):
+    """ntcb_adamw_args: one step's scalars."""
+    _fields_ = [
+        ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+        ("grad_scale", C.c_double), ("it", C.c_longlong), ("seed", C.c_uint64), ("it_dev", C.c_void_p), ("lr_dev", C.c_void_p),
+        ("grad_scale_dev", C.c_void_p),
+    ]
+
+
 _fp = C.POINTER(C.c_float)
 _dp = C.POINTER(C.c_double)
 _ip = C.POINTER(C.c_int)
@@ -186,10 +203,21 @@ SIGNATURES = {
     "ntcb_p2p_release": (None, [_vp]),
     "ntcb_p2p_set_poll_limit": (None, [_vp, C.c_uint]),
     "ntcb_p2p_barrier": (C.c_int, [_vp, C.c_uint]),
+    "ntcb_symbol_logprobs": (C.c_int, [C.POINTER(SymbolDesc), _vp, _vp, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, C.c_char_p, C.c_size_t]),
+    "ntcb_symbol_logprobs_grad": (C.c_int, [C.POINTER(SymbolDesc), _vp, _vp, _vp, _vp, _vp, C.c_longlong, _vp, C.c_longlong, _vp, C.c_longlong,
+                                            _vp, C.c_char_p, C.c_size_t]),
+    "ntcb_adamw_create": (_vp, [C.c_int, C.c_int, C.POINTER(C.c_longlong), _ip, _ip, C.c_int, C.c_char_p, C.c_size_t]),
+    "ntcb_adamw_destroy": (None, [_vp]),
+    "ntcb_adamw_state_bytes": (C.c_size_t, [_vp]),
+    "ntcb_adamw_offset": (C.c_longlong, [_vp, C.c_int]),
+    "ntcb_adamw_step": (C.c_int, [_vp, _vp, _vp, _vp, C.POINTER(AdamWArgs), _vp, C.c_char_p, C.c_size_t]),
+    "ntcb_adamw_get_moments": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_char_p, C.c_size_t]),
+    "ntcb_adamw_set_moments": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_char_p, C.c_size_t]),
 }
 
 COMM_ID_BYTES = 128   # NTCB_COMM_ID_BYTES
 P2P_HANDLE_BYTES = 64   # NTCB_P2P_HANDLE_BYTES
+MAX_TOPK = 32   # NTCB_MAX_TOPK
 
 _lib = None
 

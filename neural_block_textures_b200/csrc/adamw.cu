@@ -1,0 +1,476 @@
+// AdamW over many tensors in one launch, with the moments in 32 bits or in 8 (ntcb_adamw_*, include/ntc_b200.h).
+//
+//   g' = s g, m = b1 m + (1 - b1) g', v = b2 v + (1 - b2) g'^2, p = (1 - lr wd) p - (lr / c1) m / (sqrt(v) / sqrt(c2) + eps)
+//
+// Nothing is reduced over a tensor, so the step is bound by memory: 28 bytes per fp32 element with 32-bit moments, 16
+// with 8-bit ones. Work is cut into chunks of one tensor; a CTA takes one chunk, found in a table that the plan keeps
+// on the device, and the tensors' addresses come with the launch (by value: they may change from step to step).
+//
+// 8-bit moments. Blocks of 256 elements, one warp each. A value is held as its float's exponent and upper 3 mantissa
+// bits, q = bits >> 20, counted from the base of the block's window, which ends at the block's largest q. The grid of q
+// does not move with the block, so a value that stays is never rounded again. Rounding to nearest would freeze v (a step
+// changes it by at most 0.1 % down, a grid step is 6 to 12 %), so it is stochastic: 16 random bits are added above the
+// 4 lowest of the 20 bits that are dropped (a bias below 2^-16 of a grid step), which keeps the expected value.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "../../include/ntc_b200.h"
+#include "device_scope.h"
+#include "noise.cuh"
+
+namespace ntcb {
+namespace {
+
+constexpr int kBlock = 256;            // elements that share a window (and start a tensor's moments)
+constexpr int kChunk = 2048;           // elements of one CTA: 8 blocks, one per warp
+constexpr int kVec = 8;                // elements of one lane
+constexpr uint32_t kTopM = 126, kTopV = 254;
+constexpr uint32_t kStreamAdamW = 5;   // beside the trainer's noise streams (noise.cuh)
+constexpr unsigned kFull = 0xffffffffu;
+
+struct Chunk {
+    long long start;      // first element within the tensor
+    long long state;      // first element within the moments
+    int tensor, n;        // n <= kChunk
+    int param_type, grad_type;
+};
+
+struct Scalars {
+    double lr, beta1, beta2, wd, log_beta1, log_beta2;   // the device-scalar path recomputes step / inv / decay from these
+    float b1, omb1, b2, omb2, eps, step, inv, decay, scale;
+    uint64_t seed;
+    uint32_t it;
+    const long long* it_dev;
+    const float* lr_dev;
+    const float* scale_dev;
+};
+
+template <int N>
+struct StepArgs {
+    Scalars c;
+    const Chunk* chunks;
+    void* state;
+    long long total;
+    int first;            // tensor of p[0] / g[0]
+    void* p[N];
+    const void* g[N];
+};
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void from_f32(float v, float& o) { o = v; }
+__device__ __forceinline__ void from_f32(float v, __half& o) { o = __float2half_rn(v); }
+__device__ __forceinline__ void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
+
+// kVec elements at p, of which n are there; wide when all are and p is aligned.
+template <class T>
+__device__ __forceinline__ void load8(const T* p, int n, float (&v)[kVec]) {
+    if (n >= kVec && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        alignas(16) T e[kVec];
+        uint4 w[sizeof(e) / 16];
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(e) / 16); i++) w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+        memcpy(e, w, sizeof(e));
+#pragma unroll
+        for (int i = 0; i < kVec; i++) v[i] = to_f32(e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; i++) v[i] = i < n ? to_f32(p[i]) : 0.0f;
+    }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, int n, const float (&v)[kVec]) {
+    if (n >= kVec && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        alignas(16) T e[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; i++) from_f32(v[i], e[i]);
+        uint4 w[sizeof(e) / 16];
+        memcpy(w, e, sizeof(e));
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(e) / 16); i++) __stcs(reinterpret_cast<uint4*>(p) + i, w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; i++)
+            if (i < n) from_f32(v[i], p[i]);
+    }
+}
+__device__ __forceinline__ void load8(const void* p, int type, long long at, int n, float (&v)[kVec]) {
+    if (type == NTCB_F32) load8(static_cast<const float*>(p) + at, n, v);
+    else if (type == NTCB_F16) load8(static_cast<const __half*>(p) + at, n, v);
+    else load8(static_cast<const __nv_bfloat16*>(p) + at, n, v);
+}
+__device__ __forceinline__ void store8(void* p, int type, long long at, int n, const float (&v)[kVec]) {
+    if (type == NTCB_F32) store8(static_cast<float*>(p) + at, n, v);
+    else if (type == NTCB_F16) store8(static_cast<__half*>(p) + at, n, v);
+    else store8(static_cast<__nv_bfloat16*>(p) + at, n, v);
+}
+
+// The scalars of this step: as the host worked them out, or, with device scalars, the same expressions here.
+__device__ __forceinline__ void resolve(Scalars& c) {
+    if (c.scale_dev) c.scale *= *c.scale_dev;
+    if (!c.it_dev && !c.lr_dev) return;
+    const double it = c.it_dev ? (double)*c.it_dev : (double)c.it;
+    const double lr = c.lr_dev ? (double)*c.lr_dev : c.lr;
+    c.it = c.it_dev ? (uint32_t)*c.it_dev : c.it;
+    c.step = (float)(lr / -expm1(it * c.log_beta1));
+    c.inv = (float)(1.0 / sqrt(-expm1(it * c.log_beta2)));
+    c.decay = (float)(1.0 - lr * c.wd);
+}
+
+// Products and sums of the moments are rounded one by one (no fused multiply-add), so that the 8-bit codes follow from
+// elementary operations; the parameter's update uses CUDA's approximate square root and quotient (a few units in the
+// last place of an update that is itself a small part of the parameter).
+__device__ __forceinline__ void update(const Scalars& c, float& p, float g, float& m, float& v) {
+    g = __fmul_rn(g, c.scale);
+    m = __fadd_rn(__fmul_rn(m, c.b1), __fmul_rn(g, c.omb1));
+    v = __fadd_rn(__fmul_rn(v, c.b2), __fmul_rn(__fmul_rn(g, g), c.omb2));
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    p = fmaf(p, c.decay, -__fdividef(c.step * m, fmaf(r, c.inv, c.eps)));
+}
+
+// ---- 8-bit codes
+__device__ __forceinline__ uint32_t grid_of(float x, uint32_t round) {   // q of |x|; 0 for a value that is not finite
+    const uint32_t bits = __float_as_uint(x) & 0x7fffffffu;
+    return bits < 0x7f800000u ? min((bits + round) >> 20, 0x7f7u) : 0u;
+}
+__device__ __forceinline__ uint32_t code_m(float x, uint32_t q, uint32_t base) {
+    const uint32_t bits = __float_as_uint(x);
+    uint32_t c = q > base ? q - base : 0u;
+    if ((bits & 0x7fffffffu) >= 0x7f800000u) c = kTopM + 1;
+    return c ? c | ((bits >> 24) & 0x80u) : 0u;
+}
+__device__ __forceinline__ uint32_t code_v(float x, uint32_t q, uint32_t base) {
+    const uint32_t bits = __float_as_uint(x) & 0x7fffffffu;
+    uint32_t c = q > base ? q - base : 0u;
+    if (bits) c = max(c, 1u);
+    return bits >= 0x7f800000u ? kTopV + 1 : c;
+}
+__device__ __forceinline__ float value_m(uint32_t c, uint32_t base) {
+    const uint32_t k = c & 0x7fu;
+    const uint32_t bits = k == 0 ? 0u : k > kTopM ? 0x7fc00000u : (k + base) << 20;
+    return __uint_as_float(bits | (k ? (c & 0x80u) << 24 : 0u));
+}
+__device__ __forceinline__ float value_v(uint32_t c, uint32_t base) {
+    return __uint_as_float(c == 0 ? 0u : c > kTopV ? 0x7fc00000u : (c + base) << 20);
+}
+__device__ __forceinline__ uint32_t base_of(uint32_t q, uint32_t top) {   // the warp's window: up to its largest q
+    const uint32_t most = __reduce_max_sync(kFull, q);
+    return most > top ? most - top : 0u;
+}
+
+struct State8 {
+    uint8_t *m, *v;
+    uint16_t *mb, *vb;
+    __host__ __device__ State8(void* s, long long total)
+        : m(static_cast<uint8_t*>(s)), v(m + total), mb(reinterpret_cast<uint16_t*>(v + total)), vb(mb + total / kBlock) {}
+};
+
+// Encodes one block (a warp's 256 values, eight per lane) with the rounding words rm / rv.
+__device__ __forceinline__ void encode(const State8& s, long long at, int lane, const float (&m)[kVec], const float (&v)[kVec],
+                                       const uint32_t (&rm)[kVec], const uint32_t (&rv)[kVec]) {
+    uint32_t qm[kVec], qv[kVec], most_m = 0, most_v = 0;
+#pragma unroll
+    for (int i = 0; i < kVec; i++) {
+        qm[i] = grid_of(m[i], rm[i]); qv[i] = grid_of(v[i], rv[i]);
+        most_m = max(most_m, qm[i]); most_v = max(most_v, qv[i]);
+    }
+    const uint32_t bm = base_of(most_m, kTopM), bv = base_of(most_v, kTopV);
+    uint32_t wm[2] = {0, 0}, wv[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < kVec; i++) {
+        wm[i / 4] |= code_m(m[i], qm[i], bm) << (8 * (i % 4));
+        wv[i / 4] |= code_v(v[i], qv[i], bv) << (8 * (i % 4));
+    }
+    *reinterpret_cast<uint2*>(s.m + at + lane * kVec) = make_uint2(wm[0], wm[1]);
+    *reinterpret_cast<uint2*>(s.v + at + lane * kVec) = make_uint2(wv[0], wv[1]);
+    if (lane == 0) { s.mb[at / kBlock] = (uint16_t)bm; s.vb[at / kBlock] = (uint16_t)bv; }
+}
+__device__ __forceinline__ void decode(const State8& s, long long at, int lane, float (&m)[kVec], float (&v)[kVec]) {
+    const uint2 cm = *reinterpret_cast<const uint2*>(s.m + at + lane * kVec), cv = *reinterpret_cast<const uint2*>(s.v + at + lane * kVec);
+    const uint32_t bm = s.mb[at / kBlock], bv = s.vb[at / kBlock];
+#pragma unroll
+    for (int i = 0; i < kVec; i++) {
+        m[i] = value_m(((i < 4 ? cm.x : cm.y) >> (8 * (i % 4))) & 0xffu, bm);
+        v[i] = value_v(((i < 4 ? cv.x : cv.y) >> (8 * (i % 4))) & 0xffu, bv);
+    }
+}
+
+// ---- the kernels: a warp takes one block of 256 elements, a lane eight in a row
+template <int BITS, int N>
+__global__ void __launch_bounds__(256) k_adamw(const __grid_constant__ StepArgs<N> a) {
+    const Chunk ch = a.chunks[blockIdx.x];
+    const void* g = a.g[ch.tensor - a.first];
+    void* p = a.p[ch.tensor - a.first];
+    if (!g) return;
+    const int lane = threadIdx.x & 31, block = (threadIdx.x >> 5) * kBlock;
+    if (block >= ch.n) return;
+    Scalars c = a.c;
+    resolve(c);
+    const int n = min(kVec, max(0, ch.n - block - lane * kVec));   // this lane's elements
+    const long long at = ch.start + block + lane * kVec;
+    const long long st = ch.state + block;
+    float pv[kVec], gv[kVec], m[kVec], v[kVec];
+    load8(p, ch.param_type, at, n, pv);
+    load8(g, ch.grad_type, at, n, gv);
+    if constexpr (BITS == 32) {
+        float* sm = static_cast<float*>(a.state) + st + lane * kVec;
+        float* sv = sm + a.total;
+        load8(sm, kVec, m);
+        load8(sv, kVec, v);
+#pragma unroll
+        for (int i = 0; i < kVec; i++) update(c, pv[i], gv[i], m[i], v[i]);
+        store8(sm, n, m);
+        store8(sv, n, v);
+    } else {
+        const State8 s(a.state, a.total);
+        decode(s, st, lane, m, v);
+        uint32_t rm[kVec], rv[kVec];
+        const uint64_t key = stream_key(c.seed, kStreamAdamW, c.it, (uint32_t)ch.tensor);
+#pragma unroll
+        for (int i = 0; i < kVec; i += 2) {   // 64 random bits for two neighbours
+            const uint64_t h = draw64(key, (uint64_t)(at + i) >> 1);
+            rm[i] = ((uint32_t)h & 0xffffu) << 4; rv[i] = ((uint32_t)h >> 16) << 4;
+            rm[i + 1] = ((uint32_t)(h >> 32) & 0xffffu) << 4; rv[i + 1] = (uint32_t)(h >> 48) << 4;
+        }
+#pragma unroll
+        for (int i = 0; i < kVec; i++) {
+            update(c, pv[i], gv[i], m[i], v[i]);
+            if (i >= n) m[i] = v[i] = 0.0f;   // behind the tensor's end
+        }
+        encode(s, st, lane, m, v, rm, rv);
+    }
+    store8(p, ch.param_type, at, n, pv);
+}
+
+__global__ void __launch_bounds__(256) k_adamw_get(const State8 s, long long total, float* __restrict__ fm, float* __restrict__ fv) {
+    const int lane = threadIdx.x & 31;
+    const long long at = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * kBlock;
+    if (at >= total) return;
+    float m[kVec], v[kVec];
+    decode(s, at, lane, m, v);
+    store8(fm + at + lane * kVec, kVec, m);
+    store8(fv + at + lane * kVec, kVec, v);
+}
+__global__ void __launch_bounds__(256) k_adamw_set(const State8 s, long long total, const float* __restrict__ fm, const float* __restrict__ fv) {
+    const int lane = threadIdx.x & 31;
+    const long long at = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * kBlock;
+    if (at >= total) return;
+    float m[kVec], v[kVec];
+    load8(fm + at + lane * kVec, kVec, m);
+    load8(fv + at + lane * kVec, kVec, v);
+    uint32_t half[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; i++) half[i] = 1u << 19;
+    encode(s, at, lane, m, v, half, half);
+}
+
+}  // namespace
+}  // namespace ntcb
+
+struct ntcb_adamw {
+    int device = -1, bits = 32;
+    std::vector<long long> size, offset;       // offset has one entry more: the total
+    std::vector<int> param_type, grad_type;
+    std::vector<int> first_chunk;              // per tensor, one entry more
+    ntcb::Chunk* chunks = nullptr;             // device
+};
+
+namespace ntcb {
+namespace {
+
+template <int N>
+cudaError_t launch_step(const ntcb_adamw* a, const Scalars& c, void* const* params, const void* const* grads, void* state, int first,
+                        int count, cudaStream_t s) {
+    StepArgs<N> k;
+    k.c = c;
+    k.chunks = a->chunks + a->first_chunk[(size_t)first];
+    k.state = state;
+    k.total = a->offset.back();
+    k.first = first;
+    for (int i = 0; i < N; i++) {
+        k.p[i] = i < count ? params[first + i] : nullptr;
+        k.g[i] = i < count ? grads[first + i] : nullptr;
+    }
+    const int blocks = a->first_chunk[(size_t)(first + count)] - a->first_chunk[(size_t)first];
+    if (blocks == 0) return cudaSuccess;
+    if (a->bits == 32) k_adamw<32, N><<<(unsigned)blocks, 256, 0, s>>>(k);
+    else k_adamw<8, N><<<(unsigned)blocks, 256, 0, s>>>(k);
+    return cudaGetLastError();
+}
+
+constexpr int kMaxPerLaunch = 1984;   // two addresses each: 31 KB of the 32 KB that a launch's arguments may take
+
+}  // namespace
+}  // namespace ntcb
+
+extern "C" {
+
+ntcb_adamw* ntcb_adamw_create(int device, int ntensors, const long long* sizes, const int* param_types, const int* grad_types,
+                              int state_bits, char* why, size_t why_cap) {
+    using namespace ntcb;
+    const auto refuse = [&](const char* m) { set_why(why, why_cap, m); return static_cast<ntcb_adamw*>(nullptr); };
+    if (ntensors < 1 || !sizes || !param_types || !grad_types) return refuse("no tensors");
+    if (state_bits != 32 && state_bits != 8) return refuse("state_bits must be 32 or 8");
+    long long total = 0, chunks = 0;   // below 2^25 + ntensors chunks
+    for (int i = 0; i < ntensors; i++) {
+        if (sizes[i] < 0 || sizes[i] > (1ll << 36)) return refuse("a tensor's size is outside 0 .. 2^36");
+        if (param_types[i] < NTCB_F32 || param_types[i] > NTCB_BF16 || grad_types[i] < NTCB_F32 || grad_types[i] > NTCB_BF16)
+            return refuse("unknown type of a parameter or a gradient");
+        total += (sizes[i] + kBlock - 1) / kBlock * kBlock;
+        chunks += (sizes[i] + kChunk - 1) / kChunk;
+        if (total > (1ll << 36)) return refuse("more than 2^36 elements");
+    }
+    ntcb_adamw* a = nullptr;
+    try {
+        a = new ntcb_adamw;
+        a->bits = state_bits;
+        a->size.assign(sizes, sizes + ntensors);
+        a->param_type.assign(param_types, param_types + ntensors);
+        a->grad_type.assign(grad_types, grad_types + ntensors);
+        std::vector<Chunk> table;
+        table.reserve((size_t)chunks);
+        long long at = 0;
+        for (int i = 0; i < ntensors; i++) {
+            a->offset.push_back(at);
+            a->first_chunk.push_back((int)table.size());
+            for (long long s = 0; s < sizes[i]; s += kChunk)
+                table.push_back(Chunk{s, at + s, i, (int)std::min<long long>(kChunk, sizes[i] - s), param_types[i], grad_types[i]});
+            at += (sizes[i] + kBlock - 1) / kBlock * kBlock;
+        }
+        a->offset.push_back(at);
+        a->first_chunk.push_back((int)table.size());
+        DeviceScope scope(device, why, why_cap);
+        if (!scope.ok) { delete a; return nullptr; }
+        a->device = scope.device;
+        if (!table.empty()) {
+            cudaError_t e = cudaMalloc(&a->chunks, table.size() * sizeof(Chunk));
+            if (e == cudaSuccess) e = cudaMemcpy(a->chunks, table.data(), table.size() * sizeof(Chunk), cudaMemcpyHostToDevice);
+            if (e != cudaSuccess) {
+                cudaGetLastError();
+                DeviceScope::fail("the table of work", e, why, why_cap);
+                if (a->chunks) cudaFree(a->chunks);
+                delete a;
+                return nullptr;
+            }
+        }
+    } catch (const std::bad_alloc&) {
+        delete a;
+        return refuse("out of host memory");
+    }
+    return a;
+}
+
+void ntcb_adamw_destroy(ntcb_adamw* a) {
+    if (!a) return;
+    if (a->chunks) cudaFree(a->chunks);
+    delete a;
+}
+
+size_t ntcb_adamw_state_bytes(const ntcb_adamw* a) {
+    if (!a) return 0;
+    const size_t total = (size_t)a->offset.back();
+    return a->bits == 32 ? total * 8 : total * 2 + total / ntcb::kBlock * 4;
+}
+
+long long ntcb_adamw_offset(const ntcb_adamw* a, int tensor) {
+    return a && tensor >= 0 && (size_t)tensor < a->offset.size() ? a->offset[(size_t)tensor] : -1;
+}
+
+int ntcb_adamw_step(const ntcb_adamw* a, void* const* params, const void* const* grads, void* state, const ntcb_adamw_args* args,
+                    void* stream, char* why, size_t why_cap) {
+    using namespace ntcb;
+    const auto refuse = [&](const char* m) { set_why(why, why_cap, m); return 0; };
+    if (!a || !params || !grads || !args) return refuse("null argument");
+    const int n = (int)a->size.size();
+    if (a->offset.back() && (!state || (reinterpret_cast<uintptr_t>(state) & 255))) return refuse("the state must be a 256-byte aligned buffer");
+    if (!(args->beta1 >= 0.0 && args->beta1 < 1.0 && args->beta2 >= 0.0 && args->beta2 < 1.0)) return refuse("a beta is outside [0, 1)");
+    if (!(args->eps >= 0.0) || !(args->weight_decay >= 0.0) || std::isinf(args->eps) || std::isinf(args->weight_decay))
+        return refuse("eps and weight_decay must be finite and not negative");
+    if (!args->lr_dev && !(std::isfinite(args->lr) && args->lr >= 0.0)) return refuse("lr must be finite and not negative");
+    if (!args->it_dev && (args->it < 1 || args->it > 0xffffffffll)) return refuse("it counts from 1 and stays below 2^32");
+    for (int i = 0; i < n; i++) {
+        if (!a->size[(size_t)i] || !grads[i]) continue;
+        if (!params[i]) return refuse("null parameter");
+        const size_t ps = a->param_type[(size_t)i] == NTCB_F32 ? 4 : 2, gs = a->grad_type[(size_t)i] == NTCB_F32 ? 4 : 2;
+        if (reinterpret_cast<uintptr_t>(params[i]) % ps || reinterpret_cast<uintptr_t>(grads[i]) % gs) return refuse("a buffer is not aligned to its type");
+    }
+    DeviceScope scope(a->device, why, why_cap);
+    if (!scope.ok) return 0;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (!args->it_dev) {   // a replayed step would repeat this step's number
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(s, &cap) != cudaSuccess) { cudaGetLastError(); return refuse("the stream cannot be used"); }
+        if (cap != cudaStreamCaptureStatusNone) return refuse("a captured step must take its number from the device (it_dev)");
+    }
+    Scalars c{};
+    c.lr = args->lr; c.beta1 = args->beta1; c.beta2 = args->beta2; c.wd = args->weight_decay;
+    c.log_beta1 = std::log(args->beta1); c.log_beta2 = std::log(args->beta2);
+    c.b1 = (float)args->beta1; c.omb1 = (float)(1.0 - args->beta1);
+    c.b2 = (float)args->beta2; c.omb2 = (float)(1.0 - args->beta2);
+    c.eps = (float)args->eps; c.scale = (float)args->grad_scale;
+    if (!args->it_dev) {
+        c.step = (float)(args->lr / (1.0 - std::pow(args->beta1, (double)args->it)));
+        c.inv = (float)(1.0 / std::sqrt(1.0 - std::pow(args->beta2, (double)args->it)));
+    }
+    c.decay = (float)(1.0 - args->lr * args->weight_decay);
+    c.seed = args->seed; c.it = (uint32_t)args->it;
+    c.it_dev = args->it_dev; c.lr_dev = args->lr_dev; c.scale_dev = args->grad_scale_dev;
+    for (int first = 0; first < n; first += kMaxPerLaunch) {
+        const int count = std::min(n - first, kMaxPerLaunch);
+        const cudaError_t e = count <= 16 ? launch_step<16>(a, c, params, grads, state, first, count, s)
+                              : count <= 128 ? launch_step<128>(a, c, params, grads, state, first, count, s)
+                                             : launch_step<kMaxPerLaunch>(a, c, params, grads, state, first, count, s);
+        if (e != cudaSuccess) return scope.launched(e, why, why_cap);
+    }
+    return 1;
+}
+
+int ntcb_adamw_get_moments(const ntcb_adamw* a, const void* state, float* m, float* v, void* stream, char* why, size_t why_cap) {
+    using namespace ntcb;
+    if (!a) { set_why(why, why_cap, "null argument"); return 0; }
+    const long long total = a->offset.back();
+    if (!total) return 1;
+    if (!state || !m || !v || (reinterpret_cast<uintptr_t>(state) & 255) || ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15)) {
+        set_why(why, why_cap, "null or unaligned buffer"); return 0;
+    }
+    DeviceScope scope(a->device, why, why_cap);
+    if (!scope.ok) return 0;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (a->bits == 32) {
+        cudaError_t e = cudaMemcpyAsync(m, state, (size_t)total * 4, cudaMemcpyDeviceToDevice, s);
+        if (e == cudaSuccess) e = cudaMemcpyAsync(v, static_cast<const float*>(state) + total, (size_t)total * 4, cudaMemcpyDeviceToDevice, s);
+        return scope.launched(e, why, why_cap);
+    }
+    k_adamw_get<<<(unsigned)((total + kChunk - 1) / kChunk), 256, 0, s>>>(State8(const_cast<void*>(state), total), total, m, v);
+    return scope.launched(cudaGetLastError(), why, why_cap);
+}
+
+int ntcb_adamw_set_moments(const ntcb_adamw* a, const float* m, const float* v, void* state, void* stream, char* why, size_t why_cap) {
+    using namespace ntcb;
+    if (!a) { set_why(why, why_cap, "null argument"); return 0; }
+    const long long total = a->offset.back();
+    if (!total) return 1;
+    if (!state || !m || !v || (reinterpret_cast<uintptr_t>(state) & 255) || ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15)) {
+        set_why(why, why_cap, "null or unaligned buffer"); return 0;
+    }
+    DeviceScope scope(a->device, why, why_cap);
+    if (!scope.ok) return 0;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (a->bits == 32) {
+        cudaError_t e = cudaMemcpyAsync(state, m, (size_t)total * 4, cudaMemcpyDeviceToDevice, s);
+        if (e == cudaSuccess) e = cudaMemcpyAsync(static_cast<float*>(state) + total, v, (size_t)total * 4, cudaMemcpyDeviceToDevice, s);
+        return scope.launched(e, why, why_cap);
+    }
+    k_adamw_set<<<(unsigned)((total + kChunk - 1) / kChunk), 256, 0, s>>>(State8(state, total), total, m, v);
+    return scope.launched(cudaGetLastError(), why, why_cap);
+}
+
+}  // extern "C"

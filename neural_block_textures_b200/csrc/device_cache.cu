@@ -3,6 +3,7 @@
 // opt-in (cudaFuncSetAttribute acts on the current device's context) is kept per device ordinal, never once per
 // process. Both are safe to call from several host threads.
 #include "kernels.h"
+#include "device_scope.h"
 
 #include <map>
 #include <mutex>
@@ -27,6 +28,16 @@ int device_sm_count() {
     int n = 0;
     NTCB_CHECK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
     g_nsm[dev] = n;
+    return n;
+}
+
+int device_sm_count_or_zero(int device) {
+    std::lock_guard<std::mutex> lock(g_mu);
+    auto it = g_nsm.find(device);
+    if (it != g_nsm.end()) return it->second;
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+    g_nsm[device] = n;
     return n;
 }
 

@@ -1,0 +1,161 @@
+"""AdamW over many tensors in one launch (ntcb_adamw_*), with the moments in 32 bits or in 8: the optimiser for tensors
+that a host holds and differentiates itself (many texture models' levels and layers, a symbol model's tables), beside
+the Adam that runs inside the trainer's own steps. With weight_decay 0 it is that Adam.
+
+    opt = AdamW(params, state_bits=8, weight_decay=0.01)
+    for it in range(1, iters + 1):
+        ...                                   # gradients, in p.grad or in a list
+        opt.step(it, lr)
+
+A step runs on torch's current stream of the parameters' device, without synchronising, and writes the parameters in
+place. In a captured CUDA graph the step number comes from the device: pass `it` as an int64 tensor and advance it there.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from array import array
+
+import torch
+
+from . import abi
+from .symbols import DTYPES, _call
+
+
+class AdamW:
+    """params: contiguous float32, float16 or bfloat16 CUDA tensors on one device; kept, and written by step().
+    grad_dtype: the gradients' type where it is not the parameter's. The state (`state`, one uint8 tensor) starts at
+    zero; it can be saved and restored with state_dict() / load_state_dict()."""
+
+    def __init__(self, params, state_bits: int = 32, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 0.01, seed: int = 0, grad_dtype: torch.dtype | None = None) -> None:
+        self.h = None
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("AdamW: no parameters")
+        if state_bits not in (8, 32):
+            raise ValueError("AdamW: state_bits must be 8 or 32")
+        if not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError("AdamW: betas must be in [0, 1)")
+        if not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError("AdamW: eps and weight_decay must not be negative")
+        if grad_dtype is not None and grad_dtype not in DTYPES:
+            raise TypeError(f"AdamW: gradients must be float32, float16 or bfloat16, not {grad_dtype}")
+        for p in self.params:
+            if not isinstance(p, torch.Tensor) or p.dtype not in DTYPES:
+                raise TypeError("AdamW: parameters must be float32, float16 or bfloat16 tensors")
+            if not p.is_cuda or p.device != self.params[0].device:
+                raise ValueError("AdamW: parameters must be on one CUDA device")
+            if not p.is_contiguous():
+                raise ValueError("AdamW: parameters must be contiguous")
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("AdamW: two parameters share memory")
+        self.device = self.params[0].device
+        self.state_bits, self.betas, self.eps, self.weight_decay, self.seed = state_bits, tuple(betas), eps, weight_decay, seed
+        n = len(self.params)
+        self._shape = [(p.numel(), p.dtype, grad_dtype or p.dtype) for p in self.params]
+        self.lib = abi.load_library()
+        why = C.create_string_buffer(256)
+        self.h = self.lib.ntcb_adamw_create(
+            self.device.index, n, (C.c_longlong * n)(*[s[0] for s in self._shape]), (C.c_int * n)(*[DTYPES[s[1]] for s in self._shape]),
+            (C.c_int * n)(*[DTYPES[s[2]] for s in self._shape]), state_bits, why, 256)
+        if not self.h:
+            raise RuntimeError("AdamW: " + why.value.decode())
+        self.offsets = [int(self.lib.ntcb_adamw_offset(self.h, i)) for i in range(n + 1)]   # elements; the last is the total
+        self.state = torch.zeros(self.lib.ntcb_adamw_state_bytes(self.h), dtype=torch.uint8, device=self.device)
+
+    def close(self) -> None:
+        if getattr(self, "h", None):
+            self.lib.ntcb_adamw_destroy(self.h)
+            self.h = None
+
+    def __del__(self) -> None:
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _open(self) -> None:
+        if not self.h:
+            raise RuntimeError("AdamW: closed")
+
+    def _scalar(self, x, dtype: torch.dtype, name: str):
+        """(host value, device pointer) of a number or of a one-element device tensor."""
+        if not isinstance(x, torch.Tensor):
+            return x, None
+        if x.dtype != dtype or x.numel() != 1 or x.device != self.device:
+            raise ValueError(f"AdamW.step: {name} as a tensor must be one {dtype} on {self.device}")
+        return None, x.data_ptr()
+
+    def step(self, it, lr, grads=None, grad_scale=1.0) -> None:
+        """Step number `it` (from 1) at learning rate `lr` with the gradients `grads` (default: each p.grad) times
+        grad_scale; a None gradient leaves its tensor and moments alone. it, lr and grad_scale may be device tensors
+        (int64, float32, float32)."""
+        self._open()
+        if grads is None:
+            grads = [p.grad for p in self.params]
+        if len(grads) != len(self.params):
+            raise ValueError(f"AdamW.step: {len(self.params)} gradients are needed, not {len(grads)}")
+        device = self.device
+        pp, gg = array("Q"), array("Q")
+        for p, g, (n, dtype, grad_dtype) in zip(self.params, grads, self._shape):
+            if g is None:
+                pp.append(0)
+                gg.append(0)
+                continue
+            if p.numel() != n or p.dtype is not dtype or p.device != device or not p.is_contiguous():
+                raise ValueError("AdamW.step: a parameter's size, type, device or layout has changed")
+            if g.numel() != n or g.dtype is not grad_dtype or g.device != device or not g.is_contiguous():
+                raise ValueError(f"AdamW.step: a gradient must be a contiguous {grad_dtype} tensor of {n} elements on {device}")
+            pp.append(p.data_ptr())
+            gg.append(g.data_ptr())
+        it, it_dev = self._scalar(it, torch.int64, "it")
+        lr, lr_dev = self._scalar(lr, torch.float32, "lr")
+        scale, scale_dev = self._scalar(grad_scale, torch.float32, "grad_scale")
+        args = abi.AdamWArgs(0.0 if lr is None else lr, self.betas[0], self.betas[1], self.eps, self.weight_decay,
+                             1.0 if scale is None else scale, 0 if it is None else it, self.seed & (1 << 64) - 1, it_dev, lr_dev, scale_dev)
+        _call(self.lib.ntcb_adamw_step, "AdamW.step", self.h, pp.buffer_info()[0], gg.buffer_info()[0], self.state.data_ptr(),
+              C.byref(args), torch.cuda.current_stream(device).cuda_stream)
+
+    def moments_flat(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """(m, v) as flat float32 tensors, tensor i at offsets[i]: the state itself with 32 bits, the values that the
+        codes stand for with 8."""
+        self._open()
+        total = self.offsets[-1]
+        if self.state_bits == 32:
+            mv = self.state.view(torch.float32)
+            return mv[:total], mv[total:]
+        m = torch.empty(total, dtype=torch.float32, device=self.device)
+        v = torch.empty_like(m)
+        _call(self.lib.ntcb_adamw_get_moments, "AdamW.moments", self.h, self.state.data_ptr(), m.data_ptr(), v.data_ptr(),
+              torch.cuda.current_stream(self.device).cuda_stream)
+        return m, v
+
+    def moments(self) -> tuple[list[torch.Tensor], list[torch.Tensor]]:
+        """(m, v), each a list of float32 tensors shaped as the parameters."""
+        return tuple([flat[o:o + p.numel()].view(p.shape) for o, p in zip(self.offsets, self.params)] for flat in self.moments_flat())
+
+    def set_moments(self, m, v) -> None:
+        """Sets the moments from lists of tensors (rounded to nearest with 8-bit states)."""
+        self._open()
+        flat = []
+        for name, xs in (("m", list(m)), ("v", list(v))):
+            if len(xs) != len(self.params) or any(x.numel() != s[0] for x, s in zip(xs, self._shape)):
+                raise ValueError(f"AdamW.set_moments: {name} must have one tensor of each parameter's size")
+            f = torch.zeros(self.offsets[-1], dtype=torch.float32, device=self.device)
+            for o, x in zip(self.offsets, xs):
+                f[o:o + x.numel()].copy_(x.reshape(-1))
+            flat.append(f)
+        _call(self.lib.ntcb_adamw_set_moments, "AdamW.set_moments", self.h, flat[0].data_ptr(), flat[1].data_ptr(),
+              self.state.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream)
+
+    def state_dict(self) -> dict:
+        """The state (a copy) with what it was laid out for."""
+        return {"state_bits": self.state_bits, "sizes": [s[0] for s in self._shape], "state": self.state.clone()}
+
+    def load_state_dict(self, d: dict) -> None:
+        if d["state_bits"] != self.state_bits or list(d["sizes"]) != [s[0] for s in self._shape]:
+            raise ValueError("AdamW.load_state_dict: the state is of another layout")
+        if d["state"].dtype != torch.uint8 or d["state"].numel() != self.state.numel():
+            raise ValueError("AdamW.load_state_dict: the state has another size")
+        self.state.copy_(d["state"])

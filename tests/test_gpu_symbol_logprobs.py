@@ -1,0 +1,318 @@
+"""symbol_logprobs and its gradient against their formulas in 64 bits: row lengths around every change of kernel, types,
+strides, masks, ties, and the ways a user may call them (streams, graphs, in place, broadcast).
+
+Tolerances, from the roundings counted before the first run. A thread adds at most `seq` terms in a row and partial
+sums are joined in at most 40 more roundings; each exponential is off by 2^-22 plus 2^-23 per unit of its exponent,
+which weighed with the terms themselves is at most log V. So s is off by (seq + 40 + 8 + 4 log V) 2^-24 relatively, and
+so is log s absolutely; H adds u / s, off by the same relatively, at most log V + 1 in size."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from neural_block_textures_b200 import symbol_logprobs, symbol_logprobs_grad
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+LENGTHS = [1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 31, 57, 64, 100, 121, 128, 249, 256, 257, 505, 512, 777, 1017, 1018, 1024, 1025, 2047, 4099, 6001]
+
+
+def seq(v):
+    return 32 if v <= 1024 else -(-v // (8 * 256)) * 8 + 8
+
+
+def tol(v):
+    return (seq(v) + 48 + 4 * math.log(v)) * U
+
+
+def make(n, v, dtype, seed=0, stride=None, offset=0, symbol=torch.int64, scale=3.0, masks=True):
+    gen = torch.Generator().manual_seed(seed)
+    stride = stride or v
+    store = torch.full((n * stride + offset + 64,), 7.0, dtype=DT[dtype])
+    x = store[offset:offset + n * stride].view(n, stride)[:, :v]
+    x.copy_((torch.randn(n, v, generator=gen) * scale).to(DT[dtype]))
+    s = torch.randint(0, v, (n,), generator=gen)
+    if masks and n >= 8:
+        x[1] = -math.inf                                        # nothing left
+        x[2, : v - 1] = -math.inf                               # one logit
+        x[3, v // 2:] = torch.finfo(DT[dtype]).min              # masked by the lowest value
+        x[4] = torch.finfo(DT[dtype]).min                       # only lowest values: uniform
+        x[5, v // 2 + 1:] = -math.inf
+        x[6] = 0.5                                              # all equal
+        x[7, ::2] = -0.0                                        # signed zeros are one value
+        x[7, 1::2] = 0.0
+        s[0] = -1
+    cuda = store.cuda()
+    xc = cuda[offset:offset + n * stride].view(n, stride)[:, :v]
+    return xc, s.to(symbol).cuda(), x.double().numpy(), s.numpy()
+
+
+def reference(x, s, topk):
+    """numpy, 64 bits: (logp, entropy, lse, ids, top)."""
+    n, v = x.shape
+    logp, ent, lse = np.zeros(n), np.zeros(n), np.zeros(n)
+    ids, top = np.full((n, topk), -1), np.full((n, topk), -np.inf)
+    for r in range(n):
+        row = x[r]
+        if np.isnan(row).any() or np.isposinf(row).any():
+            logp[r] = ent[r] = lse[r] = np.nan
+            top[r] = np.nan
+        elif np.isneginf(row).all():
+            lse[r] = logp[r] = -np.inf
+        else:
+            m = row.max()
+            e = np.exp(row - m)
+            log_s = math.log(math.fsum(e))
+            lse[r] = m + log_s   # loses log_s beside the lowest finite value, in 64 bits too: the others use m and log_s
+            p = e / math.fsum(e)
+            ent[r] = -math.fsum(a * (b - m - log_s) for a, b in zip(p[p > 0], row[p > 0]))
+            logp[r] = row[s[r]] - m - log_s if 0 <= s[r] < v else 0.0
+            order = np.argsort(-row, kind="stable")[:topk]
+            order = order[row[order] > -np.inf]
+            ids[r, : len(order)] = order
+            top[r, : len(order)] = row[order] - m - log_s
+        if s[r] < 0:
+            logp[r] = 0.0
+        elif s[r] >= v:
+            logp[r] = np.nan
+    return logp, ent, lse, ids, top
+
+
+def close(got, want, atol, rtol=2 * U):
+    got, want = got.double().cpu().numpy(), np.asarray(want)
+    same = (got == want) | (np.isnan(got) & np.isnan(want))
+    with np.errstate(invalid="ignore"):
+        ok = same | (np.abs(got - want) <= atol + rtol * np.abs(want))
+    assert ok.all(), (got[~ok][:5], want[~ok][:5], np.argwhere(~ok)[:5])
+
+
+def check_forward(x, s, x64, s64, topk):
+    v = x.shape[1]
+    r = symbol_logprobs(x, s, topk=topk)
+    logp, ent, lse, ids, top = reference(x64, s64, topk)
+    t = tol(v)
+    assert np.array_equal(r.top_ids.cpu().numpy(), ids)
+    close(r.lse, lse, t)
+    close(r.logp, logp, t)
+    close(r.top_logp, top, t)
+    close(r.entropy, ent, 2 * t * (1 + math.log(v)))
+    return r
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("v", LENGTHS)
+def test_forward_lengths(v, dtype, cuda_device):
+    for topk in sorted({0, 1, min(v, 5), min(v, 32)}):
+        check_forward(*make(19, v, dtype, seed=v, symbol=torch.int32), topk)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n, v", [(1, 65536), (1, 16385), (2, 30011), (3, 65535), (9, 20000), (40, 9001), (700, 2100), (1, 300007)])
+def test_forward_long_rows(n, v, dtype, cuda_device):
+    x, s, x64, s64 = make(n, v, dtype, seed=n + v)
+    for topk in (0, 20, 32):
+        check_forward(x, s, x64, s64, topk)
+
+
+@pytest.mark.parametrize("v, stride, offset", [(5, 7, 1), (64, 69, 3), (250, 260, 5), (1000, 1003, 7), (3001, 3010, 1)])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_forward_strides_and_alignment(v, stride, offset, dtype, cuda_device):
+    x, s, x64, s64 = make(23, v, dtype, stride=stride, offset=offset, seed=3)
+    check_forward(x, s, x64, s64, min(v, 7))
+    wide = torch.stack([s, s + 1], 1)[:, 0]   # symbols two apart
+    check_forward(x, wide, x64, s64, 0)
+    one = x[9:10].expand(6, v)                # one row, six symbols
+    check_forward(one, s[:6], np.repeat(x64[9:10], 6, 0), s64[:6], min(v, 3))
+
+
+@pytest.mark.parametrize("v", [4, 40, 300, 2000, 40000])
+def test_rows_that_are_not_numbers(v, cuda_device):
+    x, s, x64, s64 = make(12, v, "f32", seed=9)
+    for r, c, bad in [(0, 0, math.nan), (3, v - 1, math.nan), (8, v // 2, math.inf), (9, v - 1, math.nan), (10, 1, math.inf)]:
+        x[r, c] = bad
+        x64[r, c] = bad
+    x[10, 2 % v] = math.inf
+    x64[10, 2 % v] = math.inf
+    r = check_forward(x, s, x64, s64, 2)
+    assert (r.top_ids[[0, 3, 8, 9, 10]] == -1).all()
+    d = symbol_logprobs_grad(x, s, r.lse, r.entropy, -1.0, 0.5)
+    assert d[[0, 3, 8, 9, 10]].isnan().all() and not d[[1, 2, 4, 5, 6, 7, 11]].isnan().any()
+
+
+@pytest.mark.parametrize("v", [4, 300, 5000])
+def test_symbols_outside_the_alphabet(v, cuda_device):
+    x, s, x64, s64 = make(5, v, "f32", seed=4)
+    s[:] = torch.tensor([-1, v, -(1 << 40), 1 << 40, v - 1])
+    r = check_forward(x, s, x64, s.cpu().numpy(), 1)
+    d = symbol_logprobs_grad(x, s, r.lse, r.entropy, 1.0)
+    assert (d[[0, 2]] == 0).all() and d[[1, 3]].isnan().all() and d[4].isfinite().all()
+
+
+@pytest.mark.parametrize("symbol", [torch.uint8, torch.int16, torch.int32, torch.int64])
+def test_symbol_types(symbol, cuda_device):
+    x, s, x64, s64 = make(33, 100, "f16", symbol=symbol, masks=False)
+    check_forward(x, s, x64, s64, 3)
+
+
+@pytest.mark.parametrize("kind", ["ascending", "descending", "equal", "two_values", "one_thread"])
+@pytest.mark.parametrize("v", [256, 1000, 5000, 65536])
+def test_alternatives_of_hard_rows(kind, v, cuda_device):
+    i = torch.arange(v)
+    x = {"ascending": i.float(), "descending": -i.float(), "equal": torch.zeros(v), "two_values": (i % 2).float(),
+         "one_thread": torch.where(i // 8 % 256 == 3, 5.0 + (i % 97).float() / 97, 0.0)}[kind] / 16.0
+    x = x.repeat(3, 1)
+    s = torch.tensor([0, v // 2, v - 1])
+    check_forward(x.cuda(), s.cuda(), x.double().numpy(), s.numpy(), 32)
+
+
+def grad_reference(x, s, dl, dh):
+    n, v = x.shape
+    dx, scale = np.zeros((n, v)), np.zeros((n, v))
+    _, ent, lse, _, _ = reference(x, s, 0)
+    for r in range(n):
+        if np.isneginf(lse[r]):
+            continue
+        lp = x[r] - lse[r]
+        p = np.exp(lp)
+        lp = np.where(p > 0, lp, 0.0)
+        a = dl[r] if s[r] >= 0 else 0.0
+        dx[r] = -p * (a + dh[r] * (lp + ent[r]))
+        # roundings: the exponent (2^-23 of its size and of lse's), the exponential, the factor, the product
+        scale[r] = p * (abs(a) + abs(dh[r]) * (np.abs(lp) + ent[r] + 1)) * (8 + 4 * np.abs(lp) + 4 * abs(lse[r])) * U
+        scale[r] += p * abs(dh[r]) * 2 * tol(v) * (1 + math.log(v))
+        if s[r] >= 0:
+            dx[r, s[r]] += a
+            scale[r, s[r]] += 2 * U * abs(a)
+    return dx, scale
+
+
+def check_grad(x, s, x64, s64, dl, dh, dtype, **kw):
+    r = symbol_logprobs(x, s)
+    got = symbol_logprobs_grad(x, s, r.lse, r.entropy, dl, dh, **kw)
+    n = len(s64)
+    full = lambda g: np.zeros(n) if g is None else g.double().cpu().numpy() if isinstance(g, torch.Tensor) else np.full(n, np.float32(g), np.float64)
+    want, scale = grad_reference(x64, s64, full(dl), full(dh))
+    info = torch.finfo(DT[dtype])
+    err = np.abs(got.double().cpu().numpy() - want)
+    bad = err > scale + np.abs(want) * info.eps / 2 + info.smallest_normal * info.eps
+    assert not bad.any(), (err[bad].max(), np.argwhere(bad)[:4])
+    assert got.dtype == DT[dtype]
+    return got
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("v", [1, 2, 4, 5, 8, 25, 64, 121, 128, 256, 500, 505, 512, 1000, 4099])
+def test_gradient(v, dtype, cuda_device):
+    x, s, x64, s64 = make(21, v, dtype, seed=v)
+    gen = torch.Generator().manual_seed(v)
+    dl, dh = torch.randn(21, generator=gen).cuda(), torch.randn(21, generator=gen).cuda()
+    check_grad(x, s, x64, s64, dl, dh, dtype)
+    check_grad(x, s, x64, s64, dl, None, dtype)
+    check_grad(x, s, x64, s64, -0.25, 0.5, dtype)
+    check_grad(x, s, x64, s64, dl[:1].expand(21), torch.stack([dh, dl], 1)[:, 0], dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("v, stride, offset", [(4, 5, 1), (63, 69, 3), (1000, 1001, 1), (5003, 5011, 7)])
+def test_gradient_strides_and_in_place(v, stride, offset, dtype, cuda_device):
+    x, s, x64, s64 = make(14, v, dtype, stride=stride, offset=offset, seed=5)
+    want = check_grad(x, s, x64, s64, -1.0, 0.1, dtype)
+    store = torch.full((14, v + 9), 3.0, dtype=DT[dtype], device="cuda")
+    check_grad(x, s, x64, s64, -1.0, 0.1, dtype, out=store[:, 4:4 + v])
+    assert (store[:, :4] == 3).all() and (store[:, 4 + v:] == 3).all()   # nothing beside the rows is written
+    r = symbol_logprobs(x, s)
+    out = symbol_logprobs_grad(x, s, r.lse, r.entropy, -1.0, 0.1, out=x)
+    assert out.data_ptr() == x.data_ptr() and torch.equal(x, want)
+
+
+def test_gradient_against_differences(cuda_device):
+    """(f(x + h e) - f(x - h e)) / 2h in 64 bits of the formula, and of the kernel along one direction."""
+    n, v, h = 6, 37, 1e-5
+    x, s, x64, s64 = make(n, v, "f32", seed=8, masks=False)
+    gen = np.random.default_rng(1)
+    dl, dh = gen.standard_normal(n), gen.standard_normal(n)
+    f = lambda y: float((dl * reference(y, s64, 0)[0] + dh * reference(y, s64, 0)[1]).sum())
+    r = symbol_logprobs(x, s)
+    got = symbol_logprobs_grad(x, s, r.lse, r.entropy, torch.tensor(dl).float().cuda(), torch.tensor(dh).float().cuda()).double().cpu().numpy()
+    for r_, c in [(0, 0), (1, 5), (2, int(s64[2])), (3, 36), (4, int(s64[4])), (5, 20)]:
+        e = np.zeros_like(x64)
+        e[r_, c] = h
+        slope = (f(x64 + e) - f(x64 - e)) / (2 * h)
+        # central differences: h^2 / 6 of the third derivative (below 20 here) and 64-bit rounding over h
+        assert abs(slope - got[r_, c]) < 20 * h * h + 1e-9 + 1e-5 * (abs(dl[r_]) + abs(dh[r_]))
+
+
+def test_empty_and_refused(cuda_device):
+    x, s, _, _ = make(9, 50, "f32")
+    r = symbol_logprobs(x[:0], s[:0], topk=4)
+    assert r.logp.shape == (0,) and r.top_ids.shape == (0, 4)
+    assert symbol_logprobs_grad(x[:0], s[:0], r.lse, r.entropy, -1.0).shape == (0, 50)
+    r = symbol_logprobs(x, s)
+    for bad in (lambda: symbol_logprobs(x, s, topk=33), lambda: symbol_logprobs(x[:, :4], s, topk=5), lambda: symbol_logprobs(x, s, topk=-1),
+                lambda: symbol_logprobs(x.t(), s[:1].expand(50)), lambda: symbol_logprobs(x, s.cpu()),
+                lambda: symbol_logprobs_grad(x, s, r.lse[:4], r.entropy, -1.0), lambda: symbol_logprobs_grad(x, s, r.lse, None, -1.0, 1.0),
+                lambda: symbol_logprobs_grad(x, s, r.lse, r.entropy, r.lse.double()),
+                lambda: symbol_logprobs_grad(x, s, r.lse, r.entropy, -1.0, out=x.half()),
+                lambda: symbol_logprobs_grad(x, s, r.lse, r.entropy, -1.0, out=x[:1].expand(9, 50))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@pytest.mark.parametrize("n, v", [(40, 4), (40, 200), (3, 20000)])
+def test_streams_and_graphs(n, v, cuda_device):
+    x, s, x64, s64 = make(n, v, "bf16", seed=2)
+    want = symbol_logprobs(x, s, topk=3)
+    dwant = symbol_logprobs_grad(x, s, want.lse, want.entropy, -1.0, 0.3)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for st in streams:   # two calls at once
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            got.append(symbol_logprobs(x, s, topk=3))
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
+    dl = torch.full((n,), -1.0, device="cuda")
+    dh = torch.full((n,), 0.3, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        r = symbol_logprobs(x, s, topk=3)
+        d = symbol_logprobs_grad(x, s, r.lse, r.entropy, dl, dh)
+    for _ in range(2):
+        r.logp.zero_()
+        d.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(r, want)) and torch.equal(d, dwant)
+    y, s2, y64, s64b = make(n, v, "bf16", seed=77)
+    x.copy_(y)
+    s.copy_(s2)
+    graph.replay()   # new inputs in the same buffers
+    fresh = symbol_logprobs(y, s2, topk=3)
+    assert all(torch.equal(a, b) for a, b in zip(r, fresh))
+
+
+def test_rows_behind_32_bits(cuda_device):
+    """Offsets past 2^32 elements: the last rows of 4.3 G logits."""
+    v = 65536
+    n = (1 << 16) + 40
+    x = torch.empty(n, v, dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator().manual_seed(1)
+    tail = (torch.randn(8, v, generator=gen) * 3).to(torch.bfloat16)
+    x[:n - 8] = 0.0
+    x[n - 8:] = tail.cuda()
+    s = torch.randint(0, v, (n,), generator=gen)
+    r = symbol_logprobs(x, s.cuda(), topk=4)
+    logp, ent, lse, ids, top = reference(tail.double().numpy(), s[n - 8:].numpy(), 4)
+    close(r.logp[n - 8:], logp, tol(v))
+    close(r.entropy[n - 8:], ent, 2 * tol(v) * (1 + math.log(v)))
+    assert np.array_equal(r.top_ids[n - 8:].cpu().numpy(), ids)
+    assert (r.top_ids[:n - 8] == torch.arange(4, device="cuda")).all()
+    close(r.lse[:n - 8], np.full(n - 8, math.log(v)), tol(v))
+    want = symbol_logprobs_grad(tail.cuda(), s[n - 8:].cuda(), r.lse[n - 8:], r.entropy[n - 8:], -1.0)
+    symbol_logprobs_grad(x, s.cuda(), r.lse, r.entropy, -1.0, out=x)
+    assert torch.equal(x[n - 8:], want)
