@@ -4,11 +4,15 @@
 // Forward, for a row x[0..V) and its symbol t:
 //   m = max x, d = x - m, s = sum e^d, u = sum e^d d
 //   lse = m + log s, logp = (x_t - m) - log s, H = log s - u / s
-// and the topk largest logits in order (value first, then the lower index). One read of the logits does all of it: m,
-// s and u are kept online (a larger maximum rescales s and u), in 32 bits whatever the logits' type.
-// Rows: no finite logit (everything masked) gives lse = logp = -inf, H = 0 and no alternatives; a NaN or +inf gives NaN.
-// Masked logits take no part: e^d is 0 for -inf and for the type's lowest value, and d is clamped at kDLow so that
-// e^d d is 0 there too, not 0 * inf; the clamp passes NaN on.
+// and the topk largest logits in order (value first, then the lower index). One read of the logits does all of it, in 32
+// bits whatever their type. Rows: no finite logit (everything masked) gives lse = logp = -inf, H = 0 and no alternatives;
+// a NaN or +inf gives NaN.
+//
+// Exponents (Scale below): e^d = 2^y with y = x L - mL in one fused multiply-add, L = log2 e and mL = m L rounded. All
+// y of a row are off by the same e0 = mL - m L, which is known exactly and put back where the row is finished, so the only
+// rounding is y's own. y is clamped at kYLow, where 2^y is 0 in 32 bits: -inf and the type's lowest value then add 0 to u,
+// not 0 * inf; the clamp passes NaN on. Two elements share an instruction (fma.f32x2) where they can: the kernels are
+// bound by instruction issue and by the exponential unit (16 a clock and SM) before they are bound by memory.
 //
 // Gradient: p_j = e^(x_j - lse); dx_j = [j = t] dlogp - p_j (dlogp + dH (x_j - lse + H)).
 #include <cuda_bf16.h>
@@ -18,6 +22,7 @@
 #include <algorithm>
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/ntc_b200.h"
 #include "device_scope.h"
@@ -25,8 +30,9 @@
 namespace ntcb {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kDLow = -150.0f;        // e^-150 is 0 in 32 bits
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kYLow = -200.0f;        // 2^-200 is 0 in 32 bits
+constexpr float kLowest = -3.402823466e38f;
 constexpr int kMaxTop = NTCB_MAX_TOPK;  // 32: one alternative per lane
 constexpr unsigned kFull = 0xffffffffu;
 constexpr float kNegInf = -INFINITY;
@@ -49,23 +55,20 @@ struct GradArgs {
     int V, sym_type, chunks;
 };
 
-// ---------------------------------------------------------------------------------------------- elements and keys
+// ------------------------------------------------------------------------------------------------------- elements
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void from_f32(float v, float& o) { o = v; }
-__device__ __forceinline__ void from_f32(float v, __half& o) { o = __float2half_rn(v); }
-__device__ __forceinline__ void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ float exp_of(float d) {   // e^d for d in [kDLow, 0]
+__device__ __forceinline__ float exp2_of(float y) {
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * kLog2e));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
     return r;
 }
 
@@ -78,64 +81,112 @@ __device__ __forceinline__ long long load_symbol(const void* p, int type, long l
     }
 }
 
-// A logit and its index as one word: larger value first, then the lower index. 0 is no logit.
-typedef unsigned long long Key;
-__device__ __forceinline__ Key key_of(float x, int idx) {
-    const uint32_t b = __float_as_uint(x + 0.0f);   // -0 and +0 are one value
-    const uint32_t o = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
-    return ((Key)o << 32) | (uint32_t)(~(uint32_t)idx);
-}
-__device__ __forceinline__ float key_value(Key k) {
-    const uint32_t o = (uint32_t)(k >> 32);
-    return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
-}
-__device__ __forceinline__ int key_index(Key k) { return (int)(~(uint32_t)k); }
+// A vector is 16 bytes of a row: VEC elements. Rows may start anywhere, so vector c of a row holds its elements
+// [c VEC - shift, (c + 1) VEC - shift) with the shift that puts vectors on 16-byte boundaries.
+template <class T> constexpr int VEC = 16 / (int)sizeof(T);
+template <class T>
+__device__ __forceinline__ int row_shift(const T* row) { return (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % VEC<T>); }
 
-// Vectors of VEC elements: 16 bytes of a 16-bit type, 32 bytes of fp32 (two loads).
-constexpr int VEC = 8;
-template <class T> struct Align { static constexpr int elems = 16 / sizeof(T); };
-
-// Loads of the forward pass go through the read-only path; the gradient may be written over its logits, so its loads
-// are ordinary ones (streamed: nothing is read twice).
+// Loads of the forward pass go through the read-only path; the gradient may be written over its logits, so its loads are
+// ordinary ones (streamed: nothing is read twice).
 template <bool READ_ONLY, class W>
 __device__ __forceinline__ W load(const W* p) {
     if constexpr (READ_ONLY) return __ldg(p);
     else return __ldcs(p);
 }
+template <class T> __device__ __forceinline__ uint32_t raw_of(T v) {
+    if constexpr (sizeof(T) == 4) return __float_as_uint(v);
+    else if constexpr (std::is_same_v<T, __half>) return __half_as_ushort(v);
+    else return __bfloat16_as_ushort(v);
+}
+template <class T> constexpr uint32_t kRawNegInf = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __half> ? 0xfc00u : 0xff80u;
 
-// Elements [j0, j0 + VEC) of a row, -inf outside [0, V). The address of j0 is 16-byte aligned by the caller's choice of
-// the shift, so a vector inside the row is loaded wide; the first and the last one element by element.
-template <bool READ_ONLY = true, class T>
-__device__ __forceinline__ void load_vec(const T* row, int j0, int V, float (&v)[VEC]) {
-    if (j0 >= 0 && j0 + VEC <= V) {
-        if constexpr (sizeof(T) == 4) {
-            const float4* w = reinterpret_cast<const float4*>(row + j0);
-            const float4 a = load<READ_ONLY>(w), b = load<READ_ONLY>(w + 1);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 a = load<READ_ONLY>(reinterpret_cast<const uint4*>(row + j0));
-            T e[VEC];
-            memcpy(e, &a, 16);
+// Elements [j0, j0 + n) of a row one by one, -inf outside [0, V), packed into 32-bit words.
+template <class T, bool READ_ONLY, int WORDS>
+__device__ __forceinline__ void load_words(const T* row, int j0, int V, uint32_t (&w)[WORDS]) {
+    constexpr int per = 4 / (int)sizeof(T);
 #pragma unroll
-            for (int i = 0; i < VEC; i++) v[i] = to_f32(e[i]);
+    for (int i = 0; i < WORDS; i++) {
+        w[i] = 0;
+#pragma unroll
+        for (int e = 0; e < per; e++) {
+            const int j = j0 + i * per + e;
+            w[i] |= (j >= 0 && j < V ? raw_of(load<READ_ONLY>(row + j)) : kRawNegInf<T>) << (16 * e);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; i++) v[i] = (j0 + i >= 0 && j0 + i < V) ? to_f32(load<READ_ONLY>(row + j0 + i)) : kNegInf;
     }
 }
-
-// How many elements before the row the first 16-byte boundary at or below its start lies.
+// The vector at element j0: one load where it lies inside the row, else its halves, else its elements.
+template <bool READ_ONLY, class T>
+__device__ __forceinline__ uint4 load_vec(const T* row, int j0, int V) {
+    constexpr int N = VEC<T>;
+    if (j0 >= 0 && j0 + N <= V) return load<READ_ONLY>(reinterpret_cast<const uint4*>(row + j0));
+    uint32_t h[2][2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int j = j0 + k * N / 2;
+        if (j >= 0 && j + N / 2 <= V) {
+            const uint2 a = load<READ_ONLY>(reinterpret_cast<const uint2*>(row + j));
+            h[k][0] = a.x; h[k][1] = a.y;
+        } else {
+            load_words<T, READ_ONLY>(row, j, V, h[k]);
+        }
+    }
+    return make_uint4(h[0][0], h[0][1], h[1][0], h[1][1]);
+}
 template <class T>
-__device__ __forceinline__ int row_shift(const T* row) { return (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % Align<T>::elems); }
+__device__ __forceinline__ void expand(const uint4& a, float (&v)[VEC<T>]) {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+        else { __half2 h; memcpy(&h, &w[i], 4); const float2 f = __half22float2(h); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+    }
+}
+template <int N> __device__ __forceinline__ float max_of(const float (&v)[N]) {
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < N; i++) m = fmaxf(m, v[i]);
+    return m;
+}
 
+// ------------------------------------------------------------------------------------------------------ a row's sums
+
+// The factors of one maximum (or lse) m: y = x L + b. Where |m| is 2^120 or more m L could overflow, and no logit but m's
+// equals can be within 2^90 of it: L = 2^-10 is exact there and keeps e^d right (1 or 0).
+struct Scale {
+    float L, b;
+    __device__ __forceinline__ explicit Scale(float m) {
+        L = fabsf(m) >= 1.329227996e36f ? 0.0009765625f : kLog2e;
+        b = -(m * L);
+    }
+    __device__ __forceinline__ float off(float m) const { return -fmaf(m, L, b); }   // mL - m L
+};
 struct Sums { float m, s, u; };
 
-// Joins two partial rows: s and u are relative to m. u = sum e^(x - m) (x - m).
+// Adds N elements (even) with the factors c to s and u (pairs of partial sums).
+template <int N>
+__device__ __forceinline__ void add_exp(const float (&x)[N], const Scale& c, float2& s, float2& u) {
+    const float2 L = make_float2(c.L, c.L), b = make_float2(c.b, c.b);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        float2 y = __ffma2_rn(make_float2(x[i], x[i + 1]), L, b);
+        y.x = max_nan(y.x, kYLow); y.y = max_nan(y.y, kYLow);
+        const float2 e = make_float2(exp2_of(y.x), exp2_of(y.y));
+        s = __fadd2_rn(s, e);
+        u = __ffma2_rn(e, y, u);
+    }
+}
+// s and u of one maximum, without the common offset and in natural units.
+__device__ __forceinline__ Sums sums_of(float m, const Scale& c, float s, float u) {
+    const float off = c.off(m);
+    return Sums{m, fmaf(s, off * kLn2, s), kLn2 * fmaf(s, off, u)};
+}
+// Joins two partial rows: s and u are relative to m.
 __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
     const float m = fmaxf(a.m, b.m);
-    const float da = max_nan(a.m - m, kDLow), db = max_nan(b.m - m, kDLow);
-    const float ea = exp_of(da), eb = exp_of(db);
+    const float da = max_nan(a.m - m, -150.0f), db = max_nan(b.m - m, -150.0f);
+    const float ea = exp2_of(da * kLog2e), eb = exp2_of(db * kLog2e);
     Sums r;
     r.m = m;
     r.s = a.s * ea + b.s * eb;
@@ -167,69 +218,163 @@ __device__ __forceinline__ void write_row(const RowArgs& a, long long r, const T
     a.entropy[r] = o.bad ? NAN : o.entropy;
     a.lse[r] = o.bad ? NAN : o.lse;
 }
-__device__ __forceinline__ void write_top(const RowArgs& a, long long r, int i, Key k, const RowOut& o) {
-    const float v = k ? key_value(k) : kNegInf;
+
+// ------------------------------------------------------------------------------------------------------------- keys
+
+// A logit and its index as one integer: larger value first, then the lower index; 0 is no logit. 16-bit logits of up to
+// 2^16 symbols fit 32 bits (one compare, one shuffle, one warp reduction), others take 64.
+template <class T, class K>
+__device__ __forceinline__ K key_of(float x, int idx) {
+    if constexpr (sizeof(K) == 4) {
+        uint32_t b;
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) b = __float_as_uint(x + 0.0f) >> 16;
+        else b = __half_as_ushort(__float2half_rn(x + 0.0f));   // exact; -0 and +0 are one value
+        const uint32_t o = b ^ ((b & 0x8000u) ? 0xffffu : 0x8000u);
+        return (o << 16) | (0xffffu - (uint32_t)idx);
+    } else {
+        const uint32_t b = __float_as_uint(x + 0.0f);
+        const uint32_t o = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+        return ((K)o << 32) | (uint32_t)(~(uint32_t)idx);
+    }
+}
+template <class T, class K>
+__device__ __forceinline__ float key_value(K k) {
+    if constexpr (sizeof(K) == 4) {
+        const uint32_t o = k >> 16, b = o ^ ((o & 0x8000u) ? 0x8000u : 0xffffu);
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) return __uint_as_float(b << 16);
+        else return __half2float(__ushort_as_half((unsigned short)b));
+    } else {
+        const uint32_t o = (uint32_t)(k >> 32);
+        return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
+    }
+}
+template <class K>
+__device__ __forceinline__ int key_index(K k) {
+    if constexpr (sizeof(K) == 4) return (int)(0xffffu - (k & 0xffffu));
+    else return (int)(~(uint32_t)k);
+}
+template <class T, class K>
+__device__ __forceinline__ void write_top(const RowArgs& a, long long r, int i, K k, const RowOut& o) {
+    const float v = k ? key_value<T, K>(k) : kNegInf;
     const bool none = o.bad || v == kNegInf;
     a.top_ids[r * a.topk + i] = none ? -1 : key_index(k);
     a.top_logp[r * a.topk + i] = o.bad ? NAN : none ? kNegInf : (v - o.m) - o.log_s;
 }
 
+// The largest key of G neighbouring lanes, in all of them.
+template <int G, class K>
+__device__ __forceinline__ K group_max(K k) {
+    if constexpr (G == 32 && sizeof(K) == 4) return __reduce_max_sync(kFull, k);
+    else if constexpr (G == 32) {
+        const uint32_t hi = (uint32_t)(k >> 32), top = __reduce_max_sync(kFull, hi);
+        return ((K)top << 32) | __reduce_max_sync(kFull, hi == top ? (uint32_t)k : 0u);
+    } else {
+#pragma unroll
+        for (int w = G / 2; w; w >>= 1) k = max(k, __shfl_xor_sync(kFull, k, w));
+        return k;
+    }
+}
+
+// Batcher's odd-even merge sort of a thread's N keys, largest first (K. E. Batcher, "Sorting networks and their
+// applications", 1968).
+template <int N, class K>
+__device__ __forceinline__ void sort_keys(K (&a)[N]) {
+#pragma unroll
+    for (int p = 1; p < N; p <<= 1)
+#pragma unroll
+        for (int k = p; k >= 1; k >>= 1)
+#pragma unroll
+            for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; i++)
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const K x = a[i + j], y = a[i + j + k];
+                        a[i + j] = max(x, y);
+                        a[i + j + k] = min(x, y);
+                    }
+}
+
+// Sorts one key per lane, largest first (bitonic).
+template <class K>
+__device__ __forceinline__ K sort32(K k, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int step = size >> 1; step; step >>= 1) {
+            const K other = __shfl_xor_sync(kFull, k, step);
+            const bool keep_max = ((lane & step) == 0) == ((lane & size) == 0);
+            k = keep_max ? max(k, other) : min(k, other);
+        }
+    return k;
+}
+// The 32 largest of two sorted lists, sorted: the larger of a[i] and b[31 - i] is a bitonic sequence of them.
+template <class K>
+__device__ __forceinline__ K merge32(K a, K b, int lane) {
+    K k = max(a, __shfl_sync(kFull, b, 31 - lane));
+#pragma unroll
+    for (int step = 16; step; step >>= 1) {
+        const K other = __shfl_xor_sync(kFull, k, step);
+        k = (lane & step) == 0 ? max(k, other) : min(k, other);
+    }
+    return k;
+}
+
 // ------------------------------------------------------------------------------------------- rows in a few registers
 
-// G lanes hold one row of up to G * E - 7 logits (a row may start in the middle of a 16-byte word) in registers: the
-// maximum is known before the exponentials, so nothing is rescaled. Alternatives are taken one at a time, each the
-// largest key over the lanes' best ones.
-template <class T, int G, int E>
+// G lanes hold one row of up to G * E elements (its shift counted in) in registers: the maximum is known before the
+// exponentials, so nothing is rescaled. Alternatives: each lane sorts its E keys, and the row's next one is the largest
+// of the lanes' first ones, which its lane then drops.
+template <class T, int G, int E, bool TOP>
 __global__ void __launch_bounds__(256) k_logprobs_lanes(const RowArgs a) {
-    static_assert(E % VEC == 0, "whole vectors");
+    constexpr int N = VEC<T>, C = E / N;
+    static_assert(E % N == 0, "whole vectors");
+    typedef typename std::conditional<sizeof(T) == 2, uint32_t, unsigned long long>::type K;
     const long long r = (long long)blockIdx.x * (256 / G) + threadIdx.x / G;
     const int lane = threadIdx.x % G;
     const bool live = r < a.rows;
     const T* row = static_cast<const T*>(a.x) + (live ? r : 0) * a.stride;
     const int shift = row_shift(row), V = live ? a.V : 0;
-    float x[E];
-    float m = -3.402823466e38f;   // a row of nothing but -inf keeps a finite maximum: d = -inf, e^d = 0
+    float x[C][N];
+    {
+        uint4 raw[C];
 #pragma unroll
-    for (int c = 0; c < E / VEC; c++) {
-        float v[VEC];
-        load_vec(row, (c * G + lane) * VEC - shift, V, v);
+        for (int c = 0; c < C; c++) raw[c] = load_vec<true>(row, (c * G + lane) * N - shift, V);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) { x[c * VEC + i] = v[i]; m = fmaxf(m, v[i]); }
+        for (int c = 0; c < C; c++) expand<T>(raw[c], x[c]);
     }
+    float m = kLowest;   // a row of nothing but -inf keeps a finite maximum: y = -inf, e^d = 0
+#pragma unroll
+    for (int c = 0; c < C; c++) m = fmaxf(m, max_of(x[c]));
 #pragma unroll
     for (int o = G / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-    Sums q{m, 0.0f, 0.0f};
+    const Scale sc(m);
+    float2 s2 = make_float2(0.0f, 0.0f), u2 = s2;
 #pragma unroll
-    for (int i = 0; i < E; i++) {
-        const float d = max_nan(x[i] - m, kDLow);
-        const float e = exp_of(d);
-        q.s += e;
-        q.u = fmaf(e, d, q.u);
-    }
+    for (int c = 0; c < C; c++) add_exp(x[c], sc, s2, u2);
+    float2 q2 = make_float2(s2.x + s2.y, u2.x + u2.y);
 #pragma unroll
-    for (int o = G / 2; o; o >>= 1) { q.s += __shfl_xor_sync(kFull, q.s, o); q.u += __shfl_xor_sync(kFull, q.u, o); }
-    const RowOut o = finish_row(q);
+    for (int o = G / 2; o; o >>= 1) q2 = __fadd2_rn(q2, make_float2(__shfl_xor_sync(kFull, q2.x, o), __shfl_xor_sync(kFull, q2.y, o)));
+    const RowOut o = finish_row(sums_of(m, sc, q2.x, q2.y));
     if (live && lane == 0) write_row(a, r, row, o);
-    if (a.topk == 0) return;
-    uint32_t taken = 0;
-    Key best = 0;
+    if constexpr (TOP) {
+        K k[E];
 #pragma unroll
-    for (int i = 0; i < E; i++) {
-        const Key k = key_of(x[i], (i / VEC * G + lane) * VEC + i % VEC - shift);
-        if (x[i] > kNegInf) best = max(best, k);
-    }
-    for (int j = 0; j < a.topk; j++) {
-        Key g = best;
+        for (int c = 0; c < C; c++)
 #pragma unroll
-        for (int w = G / 2; w; w >>= 1) g = max(g, __shfl_xor_sync(kFull, g, w));
-        if (live && lane == 0) write_top(a, r, j, g, o);
-        if (g && g == best) {
-            best = 0;
+            for (int i = 0; i < N; i++) k[c * N + i] = x[c][i] > kNegInf ? key_of<T, K>(x[c][i], (c * G + lane) * N + i - shift) : 0;
+        sort_keys(k);
+        K mine = 0;   // the alternative that this lane writes
+        for (int j = 0; j < a.topk; j++) {
+            const K g = group_max<G>(k[0]);
+            if (k[0] == g) {
 #pragma unroll
-            for (int i = 0; i < E; i++) {
-                const Key k = key_of(x[i], (i / VEC * G + lane) * VEC + i % VEC - shift);
-                if (k == g) taken |= 1u << i;
-                if (x[i] > kNegInf && !((taken >> i) & 1u)) best = max(best, k);
+                for (int i = 0; i + 1 < E; i++) k[i] = k[i + 1];
+                k[E - 1] = 0;
+            }
+            if (lane == j % G) mine = g;
+            if (j % G == G - 1 || j + 1 == a.topk) {
+                const int at = j - j % G + lane;
+                if (live && at <= j) write_top<T>(a, r, at, mine, o);
             }
         }
     }
@@ -237,41 +382,15 @@ __global__ void __launch_bounds__(256) k_logprobs_lanes(const RowArgs a) {
 
 // ------------------------------------------------------------------------------------------------------- long rows
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kCand = 512;   // candidate alternatives held in shared memory
-
-__device__ __forceinline__ Key shfl_key(Key k, int src_xor) { return __shfl_xor_sync(kFull, k, src_xor); }
-
-// Sorts one key per lane, largest first (bitonic).
-__device__ __forceinline__ Key sort32(Key k, int lane) {
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int step = size >> 1; step; step >>= 1) {
-            const Key other = shfl_key(k, step);
-            const bool keep_max = ((lane & step) == 0) == ((lane & size) == 0);
-            k = (keep_max == (k > other)) ? k : other;
-        }
-    return k;
-}
-// The 32 largest of two sorted lists, sorted: the larger of a[i] and b[31 - i] is a bitonic sequence of them.
-__device__ __forceinline__ Key merge32(Key a, Key b, int lane) {
-    const Key rb = __shfl_sync(kFull, b, 31 - lane);
-    Key k = max(a, rb);
-#pragma unroll
-    for (int step = 16; step; step >>= 1) {
-        const Key other = shfl_key(k, step);
-        k = (((lane & step) == 0) == (k > other)) ? k : other;
-    }
-    return k;
-}
-
+// Shared memory of one row's threads (W warps): partial sums, the threads' best keys, candidate alternatives.
+template <class K, int W>
 struct LongShared {
-    Sums part[kWarps];
+    static constexpr int kCand = W * 64;
+    Sums part[W];
     Sums total;                 // this CTA's part of the row
-    Key list[kWarps][32];
-    Key top[32];                // this CTA's alternatives
-    Key cand[kCand];
+    K list[W][32];
+    K top[32];                  // this CTA's alternatives
+    K cand[kCand];
     int count;
 };
 
@@ -279,122 +398,143 @@ __device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
 }
-template <class W>
-__device__ __forceinline__ W peer_load(const W* p, unsigned rank) {   // a word of another CTA's shared memory
+template <class P>
+__device__ __forceinline__ P peer_load(const P* p, unsigned rank) {   // a word of another CTA's shared memory
     const uint32_t local = (uint32_t)__cvta_generic_to_shared(p);
     uint32_t remote;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
-    W v;
-    if constexpr (sizeof(W) == 8) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(remote));
-    else asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
+    P v;
+    if constexpr (sizeof(P) == 8) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(remote));
+    else if constexpr (std::is_same_v<P, float>) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
+    else asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote));
     return v;
 }
 
-// One row per cluster of C CTAs. Vector c of the row belongs to CTA c / per, and there to thread (c - first) % kThreads.
-// Alternatives: each thread keeps its largest logit and the vector that holds it. The topk largest of the threads'
-// maxima are at least as large as the row's topk-th logit, and every logit that large lies with one of those topk
-// threads; so only their vectors are read again (from L2), by all threads together, and the few logits that pass are
-// sorted. Work that is far above that (a row of equal logits) is taken by one warp from a running list of 32.
-template <class T>
-__global__ void __launch_bounds__(kThreads) k_logprobs_long(const RowArgs a, int C) {
-    __shared__ LongShared sh;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const unsigned rank = C > 1 ? cluster_rank() : 0;
-    const long long r = blockIdx.x / (unsigned)C;
+// One row per W warps (R rows in a CTA when W = 1), or per cluster of C CTAs of one row's part each. Vector c of the row
+// belongs to CTA c / per, and there to thread (c - first) % threads; a thread reads U vectors at a time.
+// Alternatives: each thread keeps its largest logit and the group of U vectors that holds it. The topk largest of the
+// threads' maxima are at least as large as the row's topk-th logit, and every logit that large lies with one of those
+// topk threads; so only their vectors are read again (from L2), by all threads together, and the few logits that pass
+// are sorted. What is far above that (a row of equal logits) is taken by one warp from a running list of 32.
+template <class T, class K, int W, int R>
+__global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, int C) {
+    constexpr int N = VEC<T>, kThreads = 32 * W, U = 4;
+    __shared__ LongShared<K, W> shared[R];
+    LongShared<K, W>& sh = shared[R > 1 ? threadIdx.x / kThreads : 0];
+    const auto sync = [] { if constexpr (W == 1) __syncwarp(); else __syncthreads(); };
+    const int tid = threadIdx.x % kThreads, lane = tid & 31, warp = tid >> 5;
+    const unsigned rank = W > 1 && C > 1 ? cluster_rank() : 0;
+    const long long r = R > 1 ? (long long)blockIdx.x * R + threadIdx.x / kThreads : (long long)(blockIdx.x / (unsigned)C);
+    if (R > 1 && r >= a.rows) return;   // whole warps: rows of W = 1 share no barrier
     const T* row = static_cast<const T*>(a.x) + r * a.stride;
     const int shift = row_shift(row), V = a.V;
-    const int nvec = (V + shift + VEC - 1) / VEC;
+    const int nvec = (V + shift + N - 1) / N;
     const int per = (nvec + C - 1) / C, first = min(nvec, (int)rank * per), end = min(nvec, first + per);
-    Sums q{-3.402823466e38f, 0.0f, 0.0f};
-    float mine = kNegInf;   // this thread's largest logit, and its vector (the first one that holds it)
-    int at = -1;
-    for (int c = first + tid; c < end; c += kThreads) {
-        float v[VEC];
-        load_vec(row, c * VEC - shift, V, v);
-        float cm = v[0];
+    float m = kLowest, mine = kNegInf;   // the running maximum; this thread's largest logit (-inf: none)
+    int at = -1;                         // the first vector of the first group that holds it
+    Scale sc(m);
+    float2 s2 = make_float2(0.0f, 0.0f), u2 = s2;
+    for (int c = first + tid; c < end; c += U * kThreads) {
+        uint4 raw[U];
 #pragma unroll
-        for (int i = 1; i < VEC; i++) cm = fmaxf(cm, v[i]);
-        if (cm > mine) { mine = cm; at = c; }
-        if (cm > q.m) {
-            const float d = max_nan(q.m - cm, kDLow), e = exp_of(d);
-            q.u = (q.u + q.s * d) * e;
-            q.s *= e;
-            q.m = cm;
+        for (int k = 0; k < U; k++) raw[k] = load_vec<true>(row, c + k * kThreads < end ? (c + k * kThreads) * N - shift : V, V);
+        float gm = kNegInf;
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            float v[N];
+            expand<T>(raw[k], v);
+            gm = fmaxf(gm, max_of(v));
+        }
+        if (gm > mine) { mine = gm; at = c; }
+        if (gm > m) {   // y of what is summed so far moves by the difference of the b
+            const Scale to(gm);
+            const float y = max_nan(to.b - sc.b, kYLow), e = exp2_of(y);
+            u2.x = (u2.x + s2.x * y) * e; u2.y = (u2.y + s2.y * y) * e;
+            s2.x *= e; s2.y *= e;
+            m = gm;
+            sc = to;
         }
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const float d = max_nan(v[i] - q.m, kDLow);
-            const float e = exp_of(d);
-            q.s += e;
-            q.u = fmaf(e, d, q.u);
+        for (int k = 0; k < U; k++) {
+            float v[N];
+            expand<T>(raw[k], v);
+            add_exp(v, sc, s2, u2);
         }
     }
+    Sums q = sums_of(m, sc, s2.x + s2.y, u2.x + u2.y);
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-        Sums p{__shfl_xor_sync(kFull, q.m, o), __shfl_xor_sync(kFull, q.s, o), __shfl_xor_sync(kFull, q.u, o)};
+        const Sums p{__shfl_xor_sync(kFull, q.m, o), __shfl_xor_sync(kFull, q.s, o), __shfl_xor_sync(kFull, q.u, o)};
         q = join(q, p);
     }
     if (lane == 0) sh.part[warp] = q;
     if (tid == 0) sh.count = 0;
     if (a.topk) {
-        Key k = 0;
+        K k = 0;
         if (at >= 0) {
-            float v[VEC];
-            load_vec(row, at * VEC - shift, V, v);
 #pragma unroll
-            for (int i = VEC - 1; i >= 0; i--)
-                if (v[i] == mine) k = key_of(v[i], at * VEC + i - shift);
+            for (int g = U - 1; g >= 0; g--) {
+                const int c = at + g * kThreads;
+                float v[N];
+                expand<T>(load_vec<true>(row, c < end ? c * N - shift : V, V), v);
+#pragma unroll
+                for (int i = N - 1; i >= 0; i--)
+                    if (v[i] == mine) k = key_of<T, K>(v[i], c * N + i - shift);
+            }
         }
         sh.list[warp][lane] = sort32(k, lane);
     }
-    __syncthreads();
+    sync();
     if (a.topk) {
-        for (int half = kWarps / 2; half; half >>= 1) {
+#pragma unroll
+        for (int half = W / 2; half; half >>= 1) {
             if (warp < half) {
-                const Key k = merge32(sh.list[warp][lane], sh.list[warp + half][lane], lane);
+                const K k = merge32(sh.list[warp][lane], sh.list[warp + half][lane], lane);
                 __syncwarp();
                 sh.list[warp][lane] = k;
             }
-            __syncthreads();
+            sync();
         }
-        const Key least = sh.list[0][a.topk - 1];   // 0 when fewer threads than topk hold a logit
-        const int per_thread = (end - first + kThreads - 1) / kThreads;
-        for (int item = tid; item < a.topk * per_thread; item += kThreads) {
-            const Key owner = sh.list[0][item / per_thread];
-            if (!owner) continue;
-            const int c = first + ((key_index(owner) + shift) / VEC - first) % kThreads + (item % per_thread) * kThreads;
-            if (c >= end) continue;
-            float v[VEC];
-            load_vec(row, c * VEC - shift, V, v);
+        const K least = sh.list[0][a.topk - 1];   // 0 when fewer threads than topk hold a logit
+        const int per_thread = (end - first + kThreads - 1) / kThreads, items = a.topk * per_thread;
+        const auto vector_of = [&](int item) {    // the item's vector, `end` for none
+            const K owner = item < items ? sh.list[0][item / per_thread] : 0;
+            if (!owner) return end;
+            return min(end, first + ((key_index(owner) + shift) / N - first) % kThreads + (item % per_thread) * kThreads);
+        };
+        for (int item = tid; item < items; item += kThreads) {
+            const int c = vector_of(item);
+            if (c == end) continue;
+            float v[N];
+            expand<T>(load_vec<true>(row, c * N - shift, V), v);
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                const Key k = key_of(v[i], c * VEC + i - shift);
-                if (v[i] > kNegInf && k >= least) {
+            for (int i = 0; i < N; i++) {
+                if (!(v[i] > kNegInf)) continue;
+                const K k = key_of<T, K>(v[i], c * N + i - shift);
+                if (k >= least) {
                     const int p = atomicAdd(&sh.count, 1);
-                    if (p < kCand) sh.cand[p] = k;
+                    if (p < sh.kCand) sh.cand[p] = k;
                 }
             }
         }
-        __syncthreads();
+        sync();
         if (warp == 0) {
-            Key top = 0;
-            if (sh.count <= kCand) {
-                for (int i = 0; i < sh.count; i += 32) {
-                    const Key k = sort32(i + lane < sh.count ? sh.cand[i + lane] : 0, lane);
-                    top = merge32(top, k, lane);
+            K top = 0;
+            const int count = sh.count;
+            if (count <= sh.kCand) {
+                for (int i = 0; i < count; i += 32) {
+                    const K k = sort32(i + lane < count ? sh.cand[i + lane] : (K)0, lane);
+                    top = i ? merge32(top, k, lane) : k;
                 }
             } else {
-                const int items = a.topk * per_thread;
                 for (int i0 = 0; i0 < items; i0 += 32) {
-                    const int item = i0 + lane;
-                    const Key owner = item < items ? sh.list[0][item / per_thread] : 0;
-                    const int c = owner ? first + ((key_index(owner) + shift) / VEC - first) % kThreads + (item % per_thread) * kThreads : end;
-                    float v[VEC];
-                    load_vec(row, c < end ? c * VEC - shift : V, V, v);
+                    const int c = vector_of(i0 + lane);
+                    float v[N];
+                    expand<T>(load_vec<true>(row, c < end ? c * N - shift : V, V), v);
 #pragma unroll
-                    for (int i = 0; i < VEC; i++) {
-                        Key k = v[i] > kNegInf ? key_of(v[i], c * VEC + i - shift) : 0;
-                        const Key last = __shfl_sync(kFull, top, 31);
+                    for (int i = 0; i < N; i++) {
+                        K k = v[i] > kNegInf ? key_of<T, K>(v[i], c * N + i - shift) : (K)0;
+                        const K last = __shfl_sync(kFull, top, 31);
                         if (k < least || k < last) k = 0;
                         if (__any_sync(kFull, k != 0)) top = merge32(top, sort32(k, lane), lane);
                     }
@@ -403,23 +543,22 @@ __global__ void __launch_bounds__(kThreads) k_logprobs_long(const RowArgs a, int
             sh.top[lane] = top;
         }
     }
-    if (warp == 0) {
-        Sums p = lane < kWarps ? sh.part[lane] : Sums{-3.402823466e38f, 0.0f, 0.0f};
+    if (W > 1 && warp == 0) {
+        q = lane < W ? sh.part[lane] : Sums{kLowest, 0.0f, 0.0f};
 #pragma unroll
-        for (int o = kWarps / 2; o; o >>= 1) {
-            Sums b{__shfl_xor_sync(kFull, p.m, o), __shfl_xor_sync(kFull, p.s, o), __shfl_xor_sync(kFull, p.u, o)};
-            p = join(p, b);
+        for (int o = W / 2; o; o >>= 1) {
+            const Sums b{__shfl_xor_sync(kFull, q.m, o), __shfl_xor_sync(kFull, q.s, o), __shfl_xor_sync(kFull, q.u, o)};
+            q = join(q, b);
         }
-        q = p;
-        if (lane == 0) sh.total = p;
+        if (lane == 0) sh.total = q;
     }
-    if (C > 1) {
-        __syncthreads();
+    if (W > 1 && C > 1) {
+        sync();
         cluster_sync();
         if (rank == 0 && warp == 0) {
-            Key top = a.topk ? sh.top[lane] : 0;
+            K top = a.topk ? sh.top[lane] : (K)0;
             for (int w = 1; w < C; w++) {
-                Sums b{peer_load(&sh.total.m, w), peer_load(&sh.total.s, w), peer_load(&sh.total.u, w)};
+                const Sums b{peer_load(&sh.total.m, w), peer_load(&sh.total.s, w), peer_load(&sh.total.u, w)};
                 q = join(q, b);
                 if (a.topk) top = merge32(top, peer_load(&sh.top[lane], w), lane);
             }
@@ -428,116 +567,173 @@ __global__ void __launch_bounds__(kThreads) k_logprobs_long(const RowArgs a, int
         cluster_sync();   // no CTA leaves while its shared memory is read
     }
     if (rank == 0 && warp == 0) {
-        q.m = __shfl_sync(kFull, q.m, 0); q.s = __shfl_sync(kFull, q.s, 0); q.u = __shfl_sync(kFull, q.u, 0);
+        if (W > 1) { q.m = __shfl_sync(kFull, q.m, 0); q.s = __shfl_sync(kFull, q.s, 0); q.u = __shfl_sync(kFull, q.u, 0); }
         const RowOut o = finish_row(q);
         if (lane == 0) write_row(a, r, row, o);
         __syncwarp();
-        if (lane < a.topk) write_top(a, r, lane, sh.top[lane], o);
+        if (lane < a.topk) write_top<T>(a, r, lane, sh.top[lane], o);
     }
 }
 
 // -------------------------------------------------------------------------------------------------------- gradient
 
-// One thread per vector of a row (CTAs of 256 over rows * chunks): G lanes share a row when it is short, else a row
-// takes `chunks` CTAs of kThreads vectors.
-template <class T, int G>
-__global__ void __launch_bounds__(256) k_logprobs_grad(const GradArgs a) {
-    long long r;
-    int c;
-    if constexpr (G > 0) {
-        r = (long long)blockIdx.x * (256 / G) + threadIdx.x / G;
-        c = threadIdx.x % G;
-    } else {
-        r = blockIdx.x / (unsigned)a.chunks;
-        c = (int)(blockIdx.x % (unsigned)a.chunks) * 256 + threadIdx.x;
-    }
+// A thread takes M vectors of a row: 2^lg threads share a row (256 >> lg rows a CTA), or a row takes `chunks` CTAs.
+template <class T, int M, bool ENTROPY>
+__global__ void __launch_bounds__(256) k_logprobs_grad(const GradArgs a, int lg) {
+    constexpr int N = VEC<T>;
+    const int group = 1 << lg;
+    const long long r = a.chunks > 1 ? (long long)(blockIdx.x / (unsigned)a.chunks) : (long long)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
+    const int c0 = (a.chunks > 1 ? (int)(blockIdx.x % (unsigned)a.chunks) * M * 256 : 0) + (threadIdx.x & (group - 1));
     if (r >= a.rows) return;
     const T* row = static_cast<const T*>(a.x) + r * a.stride;
     T* out = static_cast<T*>(a.dx) + r * a.dx_stride;
-    const int shift = row_shift(row), j0 = c * VEC - shift, V = a.V;
-    if (j0 >= V) return;
+    const int shift = row_shift(row), V = a.V;
+    uint4 raw[M];
+#pragma unroll
+    for (int k = 0; k < M; k++) raw[k] = load_vec<false>(row, (c0 + k * group) * N - shift, V);
     const float lse = a.lse[r];
     const long long t = load_symbol(a.sym, a.sym_type, r * a.sym_stride);
     float dl = t < 0 ? 0.0f : a.dlogp[r * a.dlogp_stride];
     if (t >= V) dl = NAN;
-    const float dh = a.dentropy ? a.dentropy[r * a.dentropy_stride] : 0.0f;
-    const float h = a.dentropy ? a.entropy[r] : 0.0f;
-    float v[VEC];
-    load_vec<false>(row, j0, V, v);
     const bool empty = lse == kNegInf;
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-        const float d = max_nan(v[i] - lse, kDLow);
-        const float p = exp_of(d);
-        float g = -p * fmaf(dh, d + h, dl);
-        if (j0 + i == t) g += dl;
-        v[i] = empty ? 0.0f : g;
+    const Scale sc(empty ? 0.0f : lse);
+    const float off = sc.off(empty ? 0.0f : lse);   // p = 2^(y + off), x - lse = (y + off) ln 2
+    const float p0 = -fmaf(off, kLn2, 1.0f);        // -2^off
+    float dh = 0.0f, base = dl;
+    if constexpr (ENTROPY) {
+        dh = a.dentropy[r * a.dentropy_stride];
+        base = fmaf(dh, fmaf(off, kLn2, a.entropy[r]), dl);
+        dh *= kLn2;
     }
-    if (j0 >= 0 && j0 + VEC <= V && (reinterpret_cast<uintptr_t>(out + j0) & 15) == 0) {
-        alignas(16) T e[VEC];
+    const float2 L2 = make_float2(sc.L, sc.L), b2 = make_float2(sc.b, sc.b), dh2 = make_float2(dh * p0, dh * p0), base2 = make_float2(base * p0, base * p0);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) from_f32(v[i], e[i]);
-        uint4 w[sizeof(e) / 16];
-        memcpy(w, e, sizeof(e));
+    for (int k = 0; k < M; k++) {
+        const int j0 = (c0 + k * group) * N - shift;
+        if (j0 >= V) break;
+        float v[N];
+        expand<T>(raw[k], v);
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(e) / 16); i++) reinterpret_cast<uint4*>(out + j0)[i] = w[i];
-    } else {
+        for (int i = 0; i < N; i += 2) {
+            float2 y = __ffma2_rn(make_float2(v[i], v[i + 1]), L2, b2);
+            y.x = max_nan(y.x, kYLow); y.y = max_nan(y.y, kYLow);
+            const float2 p = make_float2(exp2_of(y.x), exp2_of(y.y));
+            const float2 g = ENTROPY ? __fmul2_rn(p, __ffma2_rn(dh2, y, base2)) : __fmul2_rn(p, base2);
+            v[i] = g.x; v[i + 1] = g.y;
+        }
+        if (t >= j0 && t < j0 + N) {
 #pragma unroll
-        for (int i = 0; i < VEC; i++)
-            if (j0 + i >= 0 && j0 + i < V) from_f32(v[i], out[j0 + i]);
+            for (int i = 0; i < N; i++)
+                if (j0 + i == t) v[i] += dl;
+        }
+        if (empty) {
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = 0.0f;
+        }
+        uint4 w;
+        if constexpr (sizeof(T) == 4) w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        else {
+            uint32_t h[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if constexpr (std::is_same_v<T, __half>) { const __half2 e = __floats2half2_rn(v[2 * i], v[2 * i + 1]); memcpy(&h[i], &e, 4); }
+                else { const __nv_bfloat162 e = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); memcpy(&h[i], &e, 4); }
+            }
+            w = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        if (j0 >= 0 && j0 + N <= V && (reinterpret_cast<uintptr_t>(out + j0) & 15) == 0) {
+            __stcs(reinterpret_cast<uint4*>(out + j0), w);
+        } else {
+            const uint32_t h[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                if (j0 + i < 0 || j0 + i >= V) continue;
+                if constexpr (sizeof(T) == 4) out[j0 + i] = v[i];
+                else { const unsigned short e = (unsigned short)(h[i / 2] >> (16 * (i % 2))); memcpy(out + j0 + i, &e, 2); }
+            }
+        }
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------- launches
 
-int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-template <class T, int G, int E>
+// The widest a row gets with its shift: rows that all start on a 16-byte boundary have none.
+template <class T>
+int row_span(const void* x, long long stride, int V) {
+    const bool even = reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride % VEC<T> == 0;
+    return even ? V : V + VEC<T> - 1;
+}
+
+template <class T, int G, int E, bool TOP>
 void launch_lanes(const RowArgs& a, cudaStream_t s) {
-    k_logprobs_lanes<T, G, E><<<(unsigned)ceil_div(a.rows, 256 / G), 256, 0, s>>>(a);
+    k_logprobs_lanes<T, G, E, TOP><<<(unsigned)ceil_div(a.rows, 256 / G), 256, 0, s>>>(a);
+}
+template <class T, class K, int W, int R>
+cudaError_t launch_long(const RowArgs& a, int C, cudaStream_t s) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(ceil_div(a.rows, R) * C));
+    cfg.blockDim = dim3(32 * W * R);
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)C; at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = C > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, k_logprobs_long<T, K, W, R>, a, C);
 }
 
 template <class T>
 cudaError_t launch_rows(const RowArgs& a, cudaStream_t s, int sms) {
-    const int span = a.V + Align<T>::elems - 1;   // a row with its part of a 16-byte word before it
-    if (span <= 8) launch_lanes<T, 1, 8>(a, s);
-    else if (span <= 16) launch_lanes<T, 2, 8>(a, s);
-    else if (span <= 32) launch_lanes<T, 4, 8>(a, s);
-    else if (span <= 64) launch_lanes<T, 8, 8>(a, s);
-    else if (span <= 128) launch_lanes<T, 16, 8>(a, s);
-    else if (span <= 256) launch_lanes<T, 32, 8>(a, s);
-    else if (span <= 512) launch_lanes<T, 32, 16>(a, s);
-    else if (span <= 1024) launch_lanes<T, 32, 32>(a, s);
-    else {
+    constexpr int N = VEC<T>;
+    const int span = row_span<T>(a.x, a.stride, a.V);
+    if (a.topk == 0 && span <= 1024) {
+        // few lanes with many logits each: a row's joins and its end are paid per lane
+        if (span <= N) launch_lanes<T, 1, N, false>(a, s);
+        else if (span <= 16) launch_lanes<T, 1, 16, false>(a, s);
+        else if (span <= 64) launch_lanes<T, 4, 16, false>(a, s);
+        else if (span <= 128) launch_lanes<T, 4, 32, false>(a, s);
+        else if (span <= 256) launch_lanes<T, 8, 32, false>(a, s);
+        else if (span <= 512) launch_lanes<T, 16, 32, false>(a, s);
+        else launch_lanes<T, 32, 32, false>(a, s);
+    } else if (a.topk && span <= 512) {
+        if (span <= N) launch_lanes<T, 1, N, true>(a, s);
+        else if (span <= 8) launch_lanes<T, 1, 8, true>(a, s);
+        else if (span <= 16) launch_lanes<T, 2, 8, true>(a, s);
+        else if (span <= 32) launch_lanes<T, 4, 8, true>(a, s);
+        else if (span <= 64) launch_lanes<T, 8, 8, true>(a, s);
+        else if (span <= 128) launch_lanes<T, 16, 8, true>(a, s);
+        else if (span <= 256) launch_lanes<T, 32, 8, true>(a, s);
+        else launch_lanes<T, 32, 16, true>(a, s);
+    } else {
+        typedef typename std::conditional<sizeof(T) == 2, uint32_t, unsigned long long>::type K;
+        if (span <= 2048) return launch_long<T, K, 1, 8>(a, 1, s);
         int C = 1;
         while (C < 8 && a.rows * C * 2 <= 4 * sms && a.V / (C * 2) >= 2048) C *= 2;
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)(a.rows * C));
-        cfg.blockDim = dim3(kThreads);
-        cfg.stream = s;
-        cudaLaunchAttribute at{};
-        at.id = cudaLaunchAttributeClusterDimension;
-        at.val.clusterDim.x = (unsigned)C; at.val.clusterDim.y = at.val.clusterDim.z = 1;
-        cfg.attrs = &at;
-        cfg.numAttrs = C > 1 ? 1 : 0;
-        return cudaLaunchKernelEx(&cfg, k_logprobs_long<T>, a, C);
+        if (sizeof(T) == 2 && a.V > 65536) return launch_long<T, unsigned long long, 8, 1>(a, C, s);
+        return launch_long<T, K, 8, 1>(a, C, s);
     }
     return cudaGetLastError();
 }
 
-template <class T>
+template <class T, bool ENTROPY>
 cudaError_t launch_grad(GradArgs a, cudaStream_t s) {
-    const int nvec = ceil_div((long long)a.V + Align<T>::elems - 1, VEC);
-    if (nvec <= 1) k_logprobs_grad<T, 1><<<(unsigned)ceil_div(a.rows, 256), 256, 0, s>>>(a);
-    else if (nvec <= 4) k_logprobs_grad<T, 4><<<(unsigned)ceil_div(a.rows, 64), 256, 0, s>>>(a);
-    else if (nvec <= 16) k_logprobs_grad<T, 16><<<(unsigned)ceil_div(a.rows, 16), 256, 0, s>>>(a);
-    else if (nvec <= 64) k_logprobs_grad<T, 64><<<(unsigned)ceil_div(a.rows, 4), 256, 0, s>>>(a);
-    else {
-        a.chunks = ceil_div(nvec, 256);
-        k_logprobs_grad<T, 0><<<(unsigned)(a.rows * a.chunks), 256, 0, s>>>(a);
+    const int nvec = (int)ceil_div(row_span<T>(a.x, a.stride, a.V), VEC<T>);
+    int lg = 0;
+    a.chunks = 1;
+    if (nvec <= 8) {
+        while ((1 << lg) < nvec) lg++;
+        k_logprobs_grad<T, 1, ENTROPY><<<(unsigned)ceil_div(a.rows, 256 >> lg), 256, 0, s>>>(a, lg);
+    } else {
+        lg = 1;
+        while (lg < 8 && (4 << lg) < nvec) lg++;
+        if (lg == 8) a.chunks = (int)ceil_div(nvec, 1024);
+        k_logprobs_grad<T, 4, ENTROPY><<<(unsigned)(a.chunks > 1 ? a.rows * a.chunks : ceil_div(a.rows, 256 >> lg)), 256, 0, s>>>(a, lg);
     }
     return cudaGetLastError();
 }
+template <class T>
+cudaError_t launch_grad(const GradArgs& a, cudaStream_t s) { return a.dentropy ? launch_grad<T, true>(a, s) : launch_grad<T, false>(a, s); }
 
 // ------------------------------------------------------------------------------------------------------ the checks
 
@@ -549,7 +745,7 @@ const char* check_desc(const ntcb_symbol_desc* d) {
     if (d->vocab < 1 || d->vocab > (1ll << 28)) return "vocab outside 1 .. 2^28";
     if (d->row_stride < 0 || (d->row_stride > 0 && d->row_stride < d->vocab)) return "row_stride between 0 and vocab: rows overlap";
     if (d->symbol_stride < 0) return "negative symbol_stride";
-    // the largest grids: one CTA per row and up to vocab / 2048 CTAs per row (gradient), below 2^31 CTAs in all
+    // the largest grids: one CTA per row, and one per 4096 logits of a row (gradient, 32 bits), below 2^31 CTAs in all
     if (d->rows > 0x7fffffffll / 8 || d->rows * ((d->vocab + 2047) / 2048 + 1) > 0x7fffffffll) return "more than 2^31 blocks of 2048 logits";
     return nullptr;
 }
