@@ -205,59 +205,59 @@ __device__ __forceinline__ RowOut finish_row(const Sums& q) {
     o.entropy = o.empty ? 0.0f : o.log_s - q.u / q.s;
     return o;
 }
-// The row's scalars, by one thread.
+// The row's scalars, by one thread; t is its symbol, fetched with the row (the logit itself is in L1 or L2 by then).
 template <class T>
-__device__ __forceinline__ void write_row(const RowArgs& a, long long r, const T* row, const RowOut& o) {
-    const long long t = load_symbol(a.sym, a.sym_type, r * a.sym_stride);
-    float lp;
-    if (t < 0) lp = 0.0f;
-    else if (t >= a.V || o.bad) lp = NAN;
-    else if (o.empty) lp = kNegInf;
-    else lp = (to_f32(row[t]) - o.m) - o.log_s;
-    a.logp[r] = lp;
+__device__ __forceinline__ void write_row(const RowArgs& a, long long r, const T* row, long long t, const RowOut& o) {
+    const float xt = t >= 0 && t < a.V ? to_f32(row[t]) : NAN;
+    a.logp[r] = t < 0 ? 0.0f : o.bad ? NAN : o.empty ? (t < a.V ? kNegInf : NAN) : (xt - o.m) - o.log_s;
     a.entropy[r] = o.bad ? NAN : o.entropy;
     a.lse[r] = o.bad ? NAN : o.lse;
 }
 
 // ------------------------------------------------------------------------------------------------------------- keys
 
-// A logit and its index as one integer: larger value first, then the lower index; 0 is no logit. 16-bit logits of up to
-// 2^16 symbols fit 32 bits (one compare, one shuffle, one warp reduction), others take 64.
+// A logit and its position as one integer: larger value first, then the lower position; 0 is no logit. The value part
+// orders as the numbers do (-0 and +0 are one): sign and magnitude turned into an offset number. 16-bit logits at up to
+// 2^16 positions fit 32 bits (one compare, one shuffle, one warp reduction), others take 64.
 template <class T, class K>
-__device__ __forceinline__ K key_of(float x, int idx) {
-    if constexpr (sizeof(K) == 4) {
-        uint32_t b;
-        if constexpr (std::is_same_v<T, __nv_bfloat16>) b = __float_as_uint(x + 0.0f) >> 16;
-        else b = __half_as_ushort(__float2half_rn(x + 0.0f));   // exact; -0 and +0 are one value
-        const uint32_t o = b ^ ((b & 0x8000u) ? 0xffffu : 0x8000u);
-        return (o << 16) | (0xffffu - (uint32_t)idx);
-    } else {
-        const uint32_t b = __float_as_uint(x + 0.0f);
-        const uint32_t o = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
-        return ((K)o << 32) | (uint32_t)(~(uint32_t)idx);
-    }
+__device__ __forceinline__ K key_of_bits(uint32_t b, uint32_t pos) {   // b: the logit's bits, at the top of the word
+    const uint32_t s = (uint32_t)((int32_t)b >> 31);
+    if constexpr (sizeof(K) == 4) return (((b & 0x7fff0000u) ^ s) - s) + (0x8000ffffu - pos);
+    else return ((K)((((b & 0x7fffffffu) ^ s) - s) + 0x80000000u) << 32) | (uint32_t)~pos;
+}
+template <class T, class K>
+__device__ __forceinline__ K key_of(float x, int pos) {
+    if constexpr (std::is_same_v<T, __half> && sizeof(K) == 4) return key_of_bits<T, K>((uint32_t)__half_as_ushort(__float2half_rn(x)) << 16, (uint32_t)pos);
+    else return key_of_bits<T, K>(__float_as_uint(x), (uint32_t)pos);
 }
 template <class T, class K>
 __device__ __forceinline__ float key_value(K k) {
-    if constexpr (sizeof(K) == 4) {
-        const uint32_t o = k >> 16, b = o ^ ((o & 0x8000u) ? 0x8000u : 0xffffu);
-        if constexpr (std::is_same_v<T, __nv_bfloat16>) return __uint_as_float(b << 16);
-        else return __half2float(__ushort_as_half((unsigned short)b));
-    } else {
-        const uint32_t o = (uint32_t)(k >> 32);
-        return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
-    }
+    uint32_t o = sizeof(K) == 4 ? (uint32_t)k & 0xffff0000u : (uint32_t)((unsigned long long)k >> 32);
+    o -= 0x80000000u;
+    const uint32_t s = (uint32_t)((int32_t)o >> 31), b = ((o ^ s) - s) | (s & 0x80000000u);
+    if constexpr (std::is_same_v<T, __half> && sizeof(K) == 4) return __half2float(__ushort_as_half((unsigned short)(b >> 16)));
+    else return __uint_as_float(b);
 }
 template <class K>
 __device__ __forceinline__ int key_index(K k) {
     if constexpr (sizeof(K) == 4) return (int)(0xffffu - (k & 0xffffu));
     else return (int)(~(uint32_t)k);
 }
+// The N keys of a vector whose first element has position pos.
 template <class T, class K>
-__device__ __forceinline__ void write_top(const RowArgs& a, long long r, int i, K k, const RowOut& o) {
+__device__ __forceinline__ void keys_of(const uint4& a, int pos, K* k) {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) k[i] = key_of_bits<T, K>(w[i], (uint32_t)(pos + i));
+        else { k[2 * i] = key_of_bits<T, K>(w[i] << 16, (uint32_t)(pos + 2 * i)); k[2 * i + 1] = key_of_bits<T, K>(w[i] & 0xffff0000u, (uint32_t)(pos + 2 * i + 1)); }
+    }
+}
+template <class T, class K>
+__device__ __forceinline__ void write_top(const RowArgs& a, long long r, int i, K k, int shift, const RowOut& o) {
     const float v = k ? key_value<T, K>(k) : kNegInf;
     const bool none = o.bad || v == kNegInf;
-    a.top_ids[r * a.topk + i] = none ? -1 : key_index(k);
+    a.top_ids[r * a.topk + i] = none ? -1 : key_index(k) - shift;
     a.top_logp[r * a.topk + i] = o.bad ? NAN : none ? kNegInf : (v - o.m) - o.log_s;
 }
 
@@ -278,7 +278,7 @@ __device__ __forceinline__ K group_max(K k) {
 // Batcher's odd-even merge sort of a thread's N keys, largest first (K. E. Batcher, "Sorting networks and their
 // applications", 1968).
 template <int N, class K>
-__device__ __forceinline__ void sort_keys(K (&a)[N]) {
+__device__ __forceinline__ void sort_keys(K* a) {
 #pragma unroll
     for (int p = 1; p < N; p <<= 1)
 #pragma unroll
@@ -292,6 +292,27 @@ __device__ __forceinline__ void sort_keys(K (&a)[N]) {
                         a[i + j] = max(x, y);
                         a[i + j + k] = min(x, y);
                     }
+}
+// The L largest of a thread's E keys, in order, into k[0 .. L): lists of L are sorted and joined by their larger halves.
+template <int E, int L, class K>
+__device__ __forceinline__ void largest_keys(K* k) {
+    if constexpr (L == 1) {
+#pragma unroll
+        for (int i = 1; i < E; i++) k[0] = max(k[0], k[i]);
+    } else {
+        sort_keys<L>(k);
+#pragma unroll
+        for (int c = L; c < E; c += L) {
+            sort_keys<L>(k + c);
+#pragma unroll
+            for (int i = 0; i < L; i++) k[i] = max(k[i], k[c + L - 1 - i]);   // bitonic
+#pragma unroll
+            for (int h = L / 2; h; h >>= 1)
+#pragma unroll
+                for (int i = 0; i < L; i++)
+                    if (!(i & h)) { const K x = k[i], y = k[i + h]; k[i] = max(x, y); k[i + h] = min(x, y); }
+        }
+    }
 }
 
 // Sorts one key per lane, largest first (bitonic).
@@ -322,9 +343,10 @@ __device__ __forceinline__ K merge32(K a, K b, int lane) {
 // ------------------------------------------------------------------------------------------- rows in a few registers
 
 // G lanes hold one row of up to G * E elements (its shift counted in) in registers: the maximum is known before the
-// exponentials, so nothing is rescaled. Alternatives: each lane sorts its E keys, and the row's next one is the largest
-// of the lanes' first ones, which its lane then drops.
-template <class T, int G, int E, bool TOP>
+// exponentials, so nothing is rescaled. Alternatives (L > 0): each lane sorts the L largest of its E keys (L = 1 for one
+// alternative, 8 for up to eight, E for more), and the row's next one is the largest of the lanes' first ones, which
+// its lane then drops.
+template <class T, int G, int E, int L>
 __global__ void __launch_bounds__(256) k_logprobs_lanes(const RowArgs a) {
     constexpr int N = VEC<T>, C = E / N;
     static_assert(E % N == 0, "whole vectors");
@@ -334,47 +356,55 @@ __global__ void __launch_bounds__(256) k_logprobs_lanes(const RowArgs a) {
     const bool live = r < a.rows;
     const T* row = static_cast<const T*>(a.x) + (live ? r : 0) * a.stride;
     const int shift = row_shift(row), V = live ? a.V : 0;
-    float x[C][N];
-    {
-        uint4 raw[C];
+    uint4 raw[C];
 #pragma unroll
-        for (int c = 0; c < C; c++) raw[c] = load_vec<true>(row, (c * G + lane) * N - shift, V);
-#pragma unroll
-        for (int c = 0; c < C; c++) expand<T>(raw[c], x[c]);
-    }
+    for (int c = 0; c < C; c++) raw[c] = load_vec<true>(row, (c * G + lane) * N - shift, V);
+    const long long t = live && lane == 0 ? load_symbol(a.sym, a.sym_type, r * a.sym_stride) : -1;
     float m = kLowest;   // a row of nothing but -inf keeps a finite maximum: y = -inf, e^d = 0
 #pragma unroll
-    for (int c = 0; c < C; c++) m = fmaxf(m, max_of(x[c]));
+    for (int c = 0; c < C; c++) {
+        float x[N];
+        expand<T>(raw[c], x);
+        m = fmaxf(m, max_of(x));
+    }
 #pragma unroll
     for (int o = G / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
     const Scale sc(m);
     float2 s2 = make_float2(0.0f, 0.0f), u2 = s2;
 #pragma unroll
-    for (int c = 0; c < C; c++) add_exp(x[c], sc, s2, u2);
+    for (int c = 0; c < C; c++) {
+        float x[N];
+        expand<T>(raw[c], x);
+        add_exp(x, sc, s2, u2);
+    }
     float2 q2 = make_float2(s2.x + s2.y, u2.x + u2.y);
 #pragma unroll
     for (int o = G / 2; o; o >>= 1) q2 = __fadd2_rn(q2, make_float2(__shfl_xor_sync(kFull, q2.x, o), __shfl_xor_sync(kFull, q2.y, o)));
     const RowOut o = finish_row(sums_of(m, sc, q2.x, q2.y));
-    if (live && lane == 0) write_row(a, r, row, o);
-    if constexpr (TOP) {
+    if (live && lane == 0) write_row(a, r, row, t, o);
+    if constexpr (L > 0) {
         K k[E];
 #pragma unroll
-        for (int c = 0; c < C; c++)
+        for (int c = 0; c < C; c++) keys_of<T>(raw[c], (c * G + lane) * N, k + c * N);
+        largest_keys<E, L>(k);
+        if constexpr (G == 1) {
 #pragma unroll
-            for (int i = 0; i < N; i++) k[c * N + i] = x[c][i] > kNegInf ? key_of<T, K>(x[c][i], (c * G + lane) * N + i - shift) : 0;
-        sort_keys(k);
-        K mine = 0;   // the alternative that this lane writes
-        for (int j = 0; j < a.topk; j++) {
-            const K g = group_max<G>(k[0]);
-            if (k[0] == g) {
+            for (int j = 0; j < L; j++)
+                if (live && j < a.topk) write_top<T>(a, r, j, k[j], shift, o);
+        } else {
+            K mine = 0;   // the alternative that this lane writes
+            for (int j = 0; j < a.topk; j++) {
+                const K g = group_max<G>(k[0]);
+                if (k[0] == g) {
 #pragma unroll
-                for (int i = 0; i + 1 < E; i++) k[i] = k[i + 1];
-                k[E - 1] = 0;
-            }
-            if (lane == j % G) mine = g;
-            if (j % G == G - 1 || j + 1 == a.topk) {
-                const int at = j - j % G + lane;
-                if (live && at <= j) write_top<T>(a, r, at, mine, o);
+                    for (int i = 0; i + 1 < L; i++) k[i] = k[i + 1];
+                    k[L - 1] = 0;
+                }
+                if (lane == j % G) mine = g;
+                if (j % G == G - 1 || j + 1 == a.topk) {
+                    const int at = j - j % G + lane;
+                    if (live && at <= j) write_top<T>(a, r, at, mine, shift, o);
+                }
             }
         }
     }
@@ -569,9 +599,9 @@ __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, i
     if (rank == 0 && warp == 0) {
         if (W > 1) { q.m = __shfl_sync(kFull, q.m, 0); q.s = __shfl_sync(kFull, q.s, 0); q.u = __shfl_sync(kFull, q.u, 0); }
         const RowOut o = finish_row(q);
-        if (lane == 0) write_row(a, r, row, o);
+        if (lane == 0) write_row(a, r, row, load_symbol(a.sym, a.sym_type, r * a.sym_stride), o);
         __syncwarp();
-        if (lane < a.topk) write_top<T>(a, r, lane, sh.top[lane], o);
+        if (lane < a.topk) write_top<T>(a, r, lane, sh.top[lane], 0, o);
     }
 }
 
@@ -665,9 +695,21 @@ int row_span(const void* x, long long stride, int V) {
     return even ? V : V + VEC<T> - 1;
 }
 
-template <class T, int G, int E, bool TOP>
+template <class T, int G, int E, int L>
 void launch_lanes(const RowArgs& a, cudaStream_t s) {
-    k_logprobs_lanes<T, G, E, TOP><<<(unsigned)ceil_div(a.rows, 256 / G), 256, 0, s>>>(a);
+    k_logprobs_lanes<T, G, E, L><<<(unsigned)ceil_div(a.rows, 256 / G), 256, 0, s>>>(a);
+}
+// Rows of up to 32 E elements: the fewest lanes that hold them (a row's joins and its end are paid per lane).
+template <class T, int E, int L>
+bool launch_lanes(const RowArgs& a, int span, cudaStream_t s) {
+    if (span <= E) launch_lanes<T, 1, E, L>(a, s);
+    else if (span <= 2 * E) launch_lanes<T, 2, E, L>(a, s);
+    else if (span <= 4 * E) launch_lanes<T, 4, E, L>(a, s);
+    else if (span <= 8 * E) launch_lanes<T, 8, E, L>(a, s);
+    else if (span <= 16 * E) launch_lanes<T, 16, E, L>(a, s);
+    else if (span <= 32 * E) launch_lanes<T, 32, E, L>(a, s);
+    else return false;
+    return true;
 }
 template <class T, class K, int W, int R>
 cudaError_t launch_long(const RowArgs& a, int C, cudaStream_t s) {
@@ -683,35 +725,42 @@ cudaError_t launch_long(const RowArgs& a, int C, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, k_logprobs_long<T, K, W, R>, a, C);
 }
 
+template <class T, class K>
+cudaError_t launch_long(const RowArgs& a, int span, cudaStream_t s, int sms) {
+    int W = 8, C = 1;
+    while (W > 1 && (span < 64 * W * VEC<T> || a.rows * W / 2 >= 32ll * sms)) W /= 2;
+    if (W == 8)
+        while (C < 8 && a.rows * C * 2 <= 4 * sms && a.V / (C * 2) >= 2048) C *= 2;
+    if (W == 1) return launch_long<T, K, 1, 4>(a, 1, s);
+    if (W == 2) return launch_long<T, K, 2, 1>(a, 1, s);
+    if (W == 4) return launch_long<T, K, 4, 1>(a, 1, s);
+    return launch_long<T, K, 8, 1>(a, C, s);
+}
+
 template <class T>
 cudaError_t launch_rows(const RowArgs& a, cudaStream_t s, int sms) {
     constexpr int N = VEC<T>;
     const int span = row_span<T>(a.x, a.stride, a.V);
-    if (a.topk == 0 && span <= 1024) {
-        // few lanes with many logits each: a row's joins and its end are paid per lane
-        if (span <= N) launch_lanes<T, 1, N, false>(a, s);
-        else if (span <= 16) launch_lanes<T, 1, 16, false>(a, s);
-        else if (span <= 64) launch_lanes<T, 4, 16, false>(a, s);
-        else if (span <= 128) launch_lanes<T, 4, 32, false>(a, s);
-        else if (span <= 256) launch_lanes<T, 8, 32, false>(a, s);
-        else if (span <= 512) launch_lanes<T, 16, 32, false>(a, s);
-        else launch_lanes<T, 32, 32, false>(a, s);
-    } else if (a.topk && span <= 512) {
-        if (span <= N) launch_lanes<T, 1, N, true>(a, s);
-        else if (span <= 8) launch_lanes<T, 1, 8, true>(a, s);
-        else if (span <= 16) launch_lanes<T, 2, 8, true>(a, s);
-        else if (span <= 32) launch_lanes<T, 4, 8, true>(a, s);
-        else if (span <= 64) launch_lanes<T, 8, 8, true>(a, s);
-        else if (span <= 128) launch_lanes<T, 16, 8, true>(a, s);
-        else if (span <= 256) launch_lanes<T, 32, 8, true>(a, s);
-        else launch_lanes<T, 32, 16, true>(a, s);
+    bool done = false;
+    if (a.topk == 0) {
+        if (span <= N) { launch_lanes<T, 1, N, 0>(a, s); done = true; }
+        else if (span <= 16) { launch_lanes<T, 1, 16, 0>(a, s); done = true; }
+        else if (span <= 64) { launch_lanes<T, 4, 16, 0>(a, s); done = true; }
+        else if (span > 64) done = launch_lanes<T, 32, 0>(a, span, s);
+    } else if (a.topk == 1) {
+        if (span <= N) { launch_lanes<T, 1, N, 1>(a, s); done = true; }
+        else done = launch_lanes<T, sizeof(T) == 2 ? 32 : 16, 1>(a, span, s);
+    } else if (a.topk <= 8) {
+        if (span <= N) { launch_lanes<T, 1, N, N>(a, s); done = true; }
+        else if (span <= 8) { launch_lanes<T, 1, 8, 8>(a, s); done = true; }
+        else done = launch_lanes<T, sizeof(T) == 2 ? 32 : 16, 8>(a, span, s);
     } else {
+        done = launch_lanes<T, 16, 16>(a, span, s);
+    }
+    if (!done) {
         typedef typename std::conditional<sizeof(T) == 2, uint32_t, unsigned long long>::type K;
-        if (span <= 2048) return launch_long<T, K, 1, 8>(a, 1, s);
-        int C = 1;
-        while (C < 8 && a.rows * C * 2 <= 4 * sms && a.V / (C * 2) >= 2048) C *= 2;
-        if (sizeof(T) == 2 && a.V > 65536) return launch_long<T, unsigned long long, 8, 1>(a, C, s);
-        return launch_long<T, K, 8, 1>(a, C, s);
+        if (sizeof(T) == 2 && a.V > 65536) return launch_long<T, unsigned long long>(a, span, s, sms);
+        return launch_long<T, K>(a, span, s, sms);
     }
     return cudaGetLastError();
 }
