@@ -18,6 +18,7 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/ntc_b200.h"
@@ -101,39 +102,52 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&v)[kVec]) {
             if (i < n) from_f32(v[i], p[i]);
     }
 }
+// The same by a type known when compiled (T) or only at run time (void).
+template <class T>
 __device__ __forceinline__ void load8(const void* p, int type, long long at, int n, float (&v)[kVec]) {
-    if (type == NTCB_F32) load8(static_cast<const float*>(p) + at, n, v);
+    if constexpr (!std::is_void_v<T>) load8(static_cast<const T*>(p) + at, n, v);
+    else if (type == NTCB_F32) load8(static_cast<const float*>(p) + at, n, v);
     else if (type == NTCB_F16) load8(static_cast<const __half*>(p) + at, n, v);
     else load8(static_cast<const __nv_bfloat16*>(p) + at, n, v);
 }
+template <class T>
 __device__ __forceinline__ void store8(void* p, int type, long long at, int n, const float (&v)[kVec]) {
-    if (type == NTCB_F32) store8(static_cast<float*>(p) + at, n, v);
+    if constexpr (!std::is_void_v<T>) store8(static_cast<T*>(p) + at, n, v);
+    else if (type == NTCB_F32) store8(static_cast<float*>(p) + at, n, v);
     else if (type == NTCB_F16) store8(static_cast<__half*>(p) + at, n, v);
     else store8(static_cast<__nv_bfloat16*>(p) + at, n, v);
 }
 
-// The scalars of this step: as the host worked them out, or, with device scalars, the same expressions here.
+// The scalars of this step: as the host worked them out, or, with device scalars, the same expressions by one thread of
+// the CTA (they take some hundred instructions in 64 bits; every warp working them out cost 40 % of an 8-bit step).
 __device__ __forceinline__ void resolve(Scalars& c) {
-    if (c.scale_dev) c.scale *= *c.scale_dev;
-    if (!c.it_dev && !c.lr_dev) return;
-    const double it = c.it_dev ? (double)*c.it_dev : (double)c.it;
-    const double lr = c.lr_dev ? (double)*c.lr_dev : c.lr;
-    c.it = c.it_dev ? (uint32_t)*c.it_dev : c.it;
-    c.step = (float)(lr / -expm1(it * c.log_beta1));
-    c.inv = (float)(1.0 / sqrt(-expm1(it * c.log_beta2)));
-    c.decay = (float)(1.0 - lr * c.wd);
+    if (!c.it_dev && !c.lr_dev && !c.scale_dev) return;
+    __shared__ float out[4];
+    if (threadIdx.x == 0) {
+        const double it = c.it_dev ? (double)*c.it_dev : (double)c.it;
+        const double lr = c.lr_dev ? (double)*c.lr_dev : c.lr;
+        out[0] = (float)(lr / -expm1(it * c.log_beta1));
+        out[1] = (float)(1.0 / sqrt(-expm1(it * c.log_beta2)));
+        out[2] = (float)(1.0 - lr * c.wd);
+        out[3] = c.scale_dev ? c.scale * *c.scale_dev : c.scale;
+    }
+    __syncthreads();
+    c.step = out[0]; c.inv = out[1]; c.decay = out[2]; c.scale = out[3];
+    if (c.it_dev) c.it = (uint32_t)*c.it_dev;
 }
 
 // Products and sums of the moments are rounded one by one (no fused multiply-add), so that the 8-bit codes follow from
-// elementary operations; the parameter's update uses CUDA's approximate square root and quotient (a few units in the
-// last place of an update that is itself a small part of the parameter).
+// elementary operations; the parameter's update uses the hardware's approximate square root and reciprocal (a few units
+// in the last place of an update that is itself a small part of the parameter).
 __device__ __forceinline__ void update(const Scalars& c, float& p, float g, float& m, float& v) {
     g = __fmul_rn(g, c.scale);
     m = __fadd_rn(__fmul_rn(m, c.b1), __fmul_rn(g, c.omb1));
     v = __fadd_rn(__fmul_rn(v, c.b2), __fmul_rn(__fmul_rn(g, g), c.omb2));
     float r;
     asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
-    p = fmaf(p, c.decay, -__fdividef(c.step * m, fmaf(r, c.inv, c.eps)));
+    r = fmaf(r, c.inv, c.eps);   // between 2^-75 (or 0) and 2^65: its reciprocal needs no care for subnormals
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r));
+    p = fmaf(p, c.decay, -(c.step * m) * r);
 }
 
 // ---- 8-bit codes
@@ -173,53 +187,129 @@ struct State8 {
         : m(static_cast<uint8_t*>(s)), v(m + total), mb(reinterpret_cast<uint16_t*>(v + total)), vb(mb + total / kBlock) {}
 };
 
-// Encodes one block (a warp's 256 values, eight per lane) with the rounding words rm / rv.
-__device__ __forceinline__ void encode(const State8& s, long long at, int lane, const float (&m)[kVec], const float (&v)[kVec],
-                                       const uint32_t (&rm)[kVec], const uint32_t (&rv)[kVec]) {
+// Where the 16 random bits of each value come from: the low half of word i is m's, the high half v's.
+struct Noise {          // two neighbouring elements share a 64-bit draw
+    uint64_t key, pair; // pair: half the index of the lane's first element (which is even)
+    __device__ __forceinline__ uint64_t operator()(int i) const { return draw64(key, pair + (uint64_t)(i / 2)); }
+};
+struct Nearest {        // half a grid step
+    __device__ __forceinline__ uint64_t operator()(int) const { return 0x8000800080008000ull; }
+};
+
+// A block with values that are not finite, or that may round to infinity: value by value. Called rarely, so it keeps its
+// arrays in local memory and off the common way's registers.
+template <class R>
+__device__ __noinline__ void encode_slow(const float* m, const float* v, R rnd, uint32_t* out) {
     uint32_t qm[kVec], qv[kVec], most_m = 0, most_v = 0;
-#pragma unroll
     for (int i = 0; i < kVec; i++) {
-        qm[i] = grid_of(m[i], rm[i]); qv[i] = grid_of(v[i], rv[i]);
+        const uint32_t w = (uint32_t)(rnd(i) >> (32 * (i % 2)));
+        qm[i] = grid_of(m[i], (w & 0xffffu) << 4); qv[i] = grid_of(v[i], (w >> 16) << 4);
         most_m = max(most_m, qm[i]); most_v = max(most_v, qv[i]);
     }
     const uint32_t bm = base_of(most_m, kTopM), bv = base_of(most_v, kTopV);
-    uint32_t wm[2] = {0, 0}, wv[2] = {0, 0};
+    for (int h = 0; h < 2; h++) {
+        uint32_t wm = 0, wv = 0;
+        for (int i = 0; i < 4; i++) {
+            wm |= code_m(m[4 * h + i], qm[4 * h + i], bm) << (8 * i);
+            wv |= code_v(v[4 * h + i], qv[4 * h + i], bv) << (8 * i);
+        }
+        out[h] = wm; out[2 + h] = wv;
+    }
+    out[4] = bm; out[5] = bv;
+}
+
+// Encodes one block (a warp's 256 values, eight per lane). The kernel is bound by integer and logic instructions (half
+// the rate of the multiply-add pipe), so the common block takes the short way: t = |bits| + (random << 4) keeps its
+// fraction, the block's largest t gives the base, and 16 (max(t, base << 20) - (base << 20)), one multiply-add, has the
+// code in its top byte. A value that is not finite, or that may round to infinity, shows in the largest t.
+template <class R>
+__device__ __forceinline__ void encode(const State8& s, long long at, int lane, const float (&m)[kVec], const float (&v)[kVec], const R& rnd) {
+    uint32_t tm[kVec], tv[kVec], most_m = 0, most_v = 0;
 #pragma unroll
-    for (int i = 0; i < kVec; i++) {
-        wm[i / 4] |= code_m(m[i], qm[i], bm) << (8 * (i % 4));
-        wv[i / 4] |= code_v(v[i], qv[i], bv) << (8 * (i % 4));
+    for (int i = 0; i < kVec; i += 2) {
+        const uint64_t r = rnd(i);
+        const uint32_t w[2] = {(uint32_t)r, (uint32_t)(r >> 32)};
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            tm[i + k] = (__float_as_uint(m[i + k]) & 0x7fffffffu) + __byte_perm(w[k], 0, 0x4410) * 16u;
+            tv[i + k] = (__float_as_uint(v[i + k]) & 0x7fffffffu) + __byte_perm(w[k], 0, 0x4432) * 16u;
+            most_m = max(most_m, tm[i + k]); most_v = max(most_v, tv[i + k]);
+        }
+    }
+    most_m = __reduce_max_sync(kFull, most_m);
+    most_v = __reduce_max_sync(kFull, most_v);
+    uint32_t wm[2], wv[2], bm, bv;
+    if (max(most_m, most_v) < 0x7f800000u) {
+        bm = most_m >> 20; bm = bm > kTopM ? bm - kTopM : 0u;
+        bv = most_v >> 20; bv = bv > kTopV ? bv - kTopV : 0u;
+        const uint32_t bm20 = bm << 20, bv20 = bv << 20;
+#pragma unroll
+        for (int i = 0; i < kVec; i++) {
+            tm[i] = (max(tm[i], bm20) * 16u - bm20 * 16u) | (__float_as_uint(m[i]) & 0x80000000u);
+            const uint32_t least = min(__float_as_uint(v[i]), 1u) * (1u << 20) + bv20;   // code 1 for v > 0
+            tv[i] = max(tv[i], least) * 16u - bv20 * 16u;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t w = __byte_perm(__byte_perm(tm[4 * h], tm[4 * h + 1], 0x0073), __byte_perm(tm[4 * h + 2], tm[4 * h + 3], 0x0073), 0x5410);
+            const uint32_t some = ((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) & 0x80808080u;   // zero carries no sign
+            wm[h] = w & (some | 0x7f7f7f7fu);
+            wv[h] = __byte_perm(__byte_perm(tv[4 * h], tv[4 * h + 1], 0x0073), __byte_perm(tv[4 * h + 2], tv[4 * h + 3], 0x0073), 0x5410);
+        }
+    } else {
+        float am[kVec], av[kVec];
+        uint32_t out[6];
+#pragma unroll
+        for (int i = 0; i < kVec; i++) { am[i] = m[i]; av[i] = v[i]; }
+        encode_slow(am, av, rnd, out);
+        wm[0] = out[0]; wm[1] = out[1]; wv[0] = out[2]; wv[1] = out[3]; bm = out[4]; bv = out[5];
     }
     *reinterpret_cast<uint2*>(s.m + at + lane * kVec) = make_uint2(wm[0], wm[1]);
     *reinterpret_cast<uint2*>(s.v + at + lane * kVec) = make_uint2(wv[0], wv[1]);
     if (lane == 0) { s.mb[at / kBlock] = (uint16_t)bm; s.vb[at / kBlock] = (uint16_t)bv; }
 }
-__device__ __forceinline__ void decode(const State8& s, long long at, int lane, float (&m)[kVec], float (&v)[kVec]) {
-    const uint2 cm = *reinterpret_cast<const uint2*>(s.m + at + lane * kVec), cv = *reinterpret_cast<const uint2*>(s.v + at + lane * kVec);
-    const uint32_t bm = s.mb[at / kBlock], bv = s.vb[at / kBlock];
+// The lane's eight values of one block: loaded (fetch) and decoded later (values), so that all loads are in flight first.
+struct Codes { uint2 m, v; uint32_t bm, bv; };
+__device__ __forceinline__ Codes fetch(const State8& s, long long at, int lane) {
+    Codes c;
+    c.m = *reinterpret_cast<const uint2*>(s.m + at + lane * kVec);
+    c.v = *reinterpret_cast<const uint2*>(s.v + at + lane * kVec);
+    c.bm = s.mb[at / kBlock]; c.bv = s.vb[at / kBlock];
+    return c;
+}
+__device__ __forceinline__ void values(const Codes& c, float (&m)[kVec], float (&v)[kVec]) {
+    const uint32_t wm[2] = {c.m.x, c.m.y}, wv[2] = {c.v.x, c.v.y};
+    const uint32_t bm20 = c.bm << 20, bv20 = c.bv << 20;
+    uint32_t nan = 0;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+        nan |= ((wm[h] & 0x7f7f7f7fu) + 0x01010101u) | (((wv[h] & 0x7f7f7f7fu) + 0x01010101u) & wv[h]);   // a top code: bit 7 of its byte
 #pragma unroll
     for (int i = 0; i < kVec; i++) {
-        m[i] = value_m(((i < 4 ? cm.x : cm.y) >> (8 * (i % 4))) & 0xffu, bm);
-        v[i] = value_v(((i < 4 ? cv.x : cv.y) >> (8 * (i % 4))) & 0xffu, bv);
+        const uint32_t tm = __byte_perm(wm[i / 4], 0, 0x4044 | ((i % 4) << 8)), k = tm & 0x7f0000u;   // the byte at bit 16
+        const uint32_t xm = (k * 16u + bm20) | ((tm * 256u) & 0x80000000u);
+        m[i] = __uint_as_float(k ? xm : 0u);
+        const uint32_t tv = __byte_perm(wv[i / 4], 0, 0x4044 | ((i % 4) << 8));
+        v[i] = __uint_as_float(tv ? tv * 16u + bv20 : 0u);
+    }
+    if (nan & 0x80808080u) {
+#pragma unroll
+        for (int i = 0; i < kVec; i++) {
+            m[i] = value_m((wm[i / 4] >> (8 * (i % 4))) & 0xffu, c.bm);
+            v[i] = value_v((wv[i / 4] >> (8 * (i % 4))) & 0xffu, c.bv);
+        }
     }
 }
 
 // ---- the kernels: a warp takes one block of 256 elements, a lane eight in a row
-template <int BITS, int N>
-__global__ void __launch_bounds__(256) k_adamw(const __grid_constant__ StepArgs<N> a) {
-    const Chunk ch = a.chunks[blockIdx.x];
-    const void* g = a.g[ch.tensor - a.first];
-    void* p = a.p[ch.tensor - a.first];
-    if (!g) return;
-    const int lane = threadIdx.x & 31, block = (threadIdx.x >> 5) * kBlock;
-    if (block >= ch.n) return;
-    Scalars c = a.c;
-    resolve(c);
+template <int BITS, class P, class G, int N>
+__device__ __forceinline__ void step_block(const StepArgs<N>& a, const Scalars& c, const Chunk& ch, void* p, const void* g, int lane, int block) {
     const int n = min(kVec, max(0, ch.n - block - lane * kVec));   // this lane's elements
     const long long at = ch.start + block + lane * kVec;
     const long long st = ch.state + block;
     float pv[kVec], gv[kVec], m[kVec], v[kVec];
-    load8(p, ch.param_type, at, n, pv);
-    load8(g, ch.grad_type, at, n, gv);
+    load8<P>(p, ch.param_type, at, n, pv);
+    load8<G>(g, ch.grad_type, at, n, gv);
     if constexpr (BITS == 32) {
         float* sm = static_cast<float*>(a.state) + st + lane * kVec;
         float* sv = sm + a.total;
@@ -229,25 +319,37 @@ __global__ void __launch_bounds__(256) k_adamw(const __grid_constant__ StepArgs<
         for (int i = 0; i < kVec; i++) update(c, pv[i], gv[i], m[i], v[i]);
         store8(sm, n, m);
         store8(sv, n, v);
+        store8<P>(p, ch.param_type, at, n, pv);
     } else {
         const State8 s(a.state, a.total);
-        decode(s, st, lane, m, v);
-        uint32_t rm[kVec], rv[kVec];
-        const uint64_t key = stream_key(c.seed, kStreamAdamW, c.it, (uint32_t)ch.tensor);
+        const Codes codes = fetch(s, st, lane);
+        values(codes, m, v);
 #pragma unroll
-        for (int i = 0; i < kVec; i += 2) {   // 64 random bits for two neighbours
-            const uint64_t h = draw64(key, (uint64_t)(at + i) >> 1);
-            rm[i] = ((uint32_t)h & 0xffffu) << 4; rv[i] = ((uint32_t)h >> 16) << 4;
-            rm[i + 1] = ((uint32_t)(h >> 32) & 0xffffu) << 4; rv[i + 1] = (uint32_t)(h >> 48) << 4;
-        }
+        for (int i = 0; i < kVec; i++) update(c, pv[i], gv[i], m[i], v[i]);
+        store8<P>(p, ch.param_type, at, n, pv);
+        if (n < kVec) {
 #pragma unroll
-        for (int i = 0; i < kVec; i++) {
-            update(c, pv[i], gv[i], m[i], v[i]);
-            if (i >= n) m[i] = v[i] = 0.0f;   // behind the tensor's end
+            for (int i = 0; i < kVec; i++)
+                if (i >= n) m[i] = v[i] = 0.0f;   // behind the tensor's end
         }
-        encode(s, st, lane, m, v, rm, rv);
+        encode(s, st, lane, m, v, Noise{stream_key(c.seed, kStreamAdamW, c.it, (uint32_t)ch.tensor), (uint64_t)at >> 1});
     }
-    store8(p, ch.param_type, at, n, pv);
+}
+
+// Parameters and gradients of one type are the usual case and take the compiled conversions; mixed ones choose per load.
+template <int BITS, int N>
+__global__ void __launch_bounds__(256, 4) k_adamw(const __grid_constant__ StepArgs<N> a) {
+    const Chunk ch = a.chunks[blockIdx.x];
+    const void* g = a.g[ch.tensor - a.first];
+    void* p = a.p[ch.tensor - a.first];
+    if (!g) return;
+    Scalars c = a.c;
+    resolve(c);
+    const int lane = threadIdx.x & 31, block = (threadIdx.x >> 5) * kBlock;
+    if (block >= ch.n) return;
+    if (ch.param_type == NTCB_F32 && ch.grad_type == NTCB_F32) step_block<BITS, float, float>(a, c, ch, p, g, lane, block);
+    else if (ch.param_type == NTCB_BF16 && ch.grad_type == NTCB_BF16) step_block<BITS, __nv_bfloat16, __nv_bfloat16>(a, c, ch, p, g, lane, block);
+    else step_block<BITS, void, void>(a, c, ch, p, g, lane, block);
 }
 
 __global__ void __launch_bounds__(256) k_adamw_get(const State8 s, long long total, float* __restrict__ fm, float* __restrict__ fv) {
@@ -255,7 +357,7 @@ __global__ void __launch_bounds__(256) k_adamw_get(const State8 s, long long tot
     const long long at = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * kBlock;
     if (at >= total) return;
     float m[kVec], v[kVec];
-    decode(s, at, lane, m, v);
+    values(fetch(s, at, lane), m, v);
     store8(fm + at + lane * kVec, kVec, m);
     store8(fv + at + lane * kVec, kVec, v);
 }
@@ -266,10 +368,7 @@ __global__ void __launch_bounds__(256) k_adamw_set(const State8 s, long long tot
     float m[kVec], v[kVec];
     load8(fm + at + lane * kVec, kVec, m);
     load8(fv + at + lane * kVec, kVec, v);
-    uint32_t half[kVec];
-#pragma unroll
-    for (int i = 0; i < kVec; i++) half[i] = 1u << 19;
-    encode(s, at, lane, m, v, half, half);
+    encode(s, at, lane, m, v, Nearest{});
 }
 
 }  // namespace
