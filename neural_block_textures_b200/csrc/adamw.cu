@@ -30,7 +30,7 @@ namespace {
 
 constexpr int kBlock = 256;            // elements that share a window (and start a tensor's moments)
 constexpr int kChunk = 2048;           // elements of one CTA: 8 blocks, one per warp
-constexpr int kVec = 8;                // elements of one lane
+constexpr int kVec = 8;                // elements of one lane (two quads)
 constexpr uint32_t kTopM = 126, kTopV = 254;
 constexpr uint32_t kStreamAdamW = 5;   // beside the trainer's noise streams (noise.cuh)
 constexpr unsigned kFull = 0xffffffffu;
@@ -44,7 +44,7 @@ struct Chunk {
 
 struct Scalars {
     double lr, beta1, beta2, wd, log_beta1, log_beta2;   // the device-scalar path recomputes step / inv / decay from these
-    float b1, omb1, b2, omb2, eps, step, inv, decay, scale;
+    float b1, omb1, b2, omb2, eps, step, inv, decay, scale, one;
     uint64_t seed;
     uint32_t it;
     const long long* it_dev;
@@ -70,36 +70,47 @@ __device__ __forceinline__ void from_f32(float v, float& o) { o = v; }
 __device__ __forceinline__ void from_f32(float v, __half& o) { o = __float2half_rn(v); }
 __device__ __forceinline__ void from_f32(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 
-// kVec elements at p, of which n are there; wide when all are and p is aligned.
+// A lane holds two quads of its warp's block: elements lane * 4 .. + 3 and 128 + lane * 4 .. + 3, so that a warp's loads and
+// stores are whole lines whatever the type. `left` is how many elements of the block exist; a quad is moved in one
+// piece where all of it does and its address allows.
 template <class T>
-__device__ __forceinline__ void load8(const T* p, int n, float (&v)[kVec]) {
-    if (n >= kVec && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-        alignas(16) T e[kVec];
-        uint4 w[sizeof(e) / 16];
+__device__ __forceinline__ void load8(const T* p, int left, float (&v)[kVec]) {
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(e) / 16); i++) w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-        memcpy(e, w, sizeof(e));
+    for (int h = 0; h < 2; h++) {
+        const T* q = p + 128 * h;
+        const int n = left - 128 * h;
+        if (n >= 4 && (reinterpret_cast<uintptr_t>(q) & (4 * sizeof(T) - 1)) == 0) {
+            typedef typename std::conditional<sizeof(T) == 4, uint4, uint2>::type W;
+            const W w = __ldcs(reinterpret_cast<const W*>(q));
+            alignas(16) T e[4];
+            memcpy(e, &w, sizeof(w));
 #pragma unroll
-        for (int i = 0; i < kVec; i++) v[i] = to_f32(e[i]);
-    } else {
+            for (int i = 0; i < 4; i++) v[4 * h + i] = to_f32(e[i]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kVec; i++) v[i] = i < n ? to_f32(p[i]) : 0.0f;
+            for (int i = 0; i < 4; i++) v[4 * h + i] = i < n ? to_f32(q[i]) : 0.0f;
+        }
     }
 }
 template <class T>
-__device__ __forceinline__ void store8(T* p, int n, const float (&v)[kVec]) {
-    if (n >= kVec && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-        alignas(16) T e[kVec];
+__device__ __forceinline__ void store8(T* p, int left, const float (&v)[kVec]) {
 #pragma unroll
-        for (int i = 0; i < kVec; i++) from_f32(v[i], e[i]);
-        uint4 w[sizeof(e) / 16];
-        memcpy(w, e, sizeof(e));
+    for (int h = 0; h < 2; h++) {
+        T* q = p + 128 * h;
+        const int n = left - 128 * h;
+        if (n >= 4 && (reinterpret_cast<uintptr_t>(q) & (4 * sizeof(T) - 1)) == 0) {
+            typedef typename std::conditional<sizeof(T) == 4, uint4, uint2>::type W;
+            alignas(16) T e[4];
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(e) / 16); i++) __stcs(reinterpret_cast<uint4*>(p) + i, w[i]);
-    } else {
+            for (int i = 0; i < 4; i++) from_f32(v[4 * h + i], e[i]);
+            W w;
+            memcpy(&w, e, sizeof(w));
+            __stcs(reinterpret_cast<W*>(q), w);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kVec; i++)
-            if (i < n) from_f32(v[i], p[i]);
+            for (int i = 0; i < 4; i++)
+                if (i < n) from_f32(v[4 * h + i], q[i]);
+        }
     }
 }
 // The same by a type known when compiled (T) or only at run time (void).
@@ -139,15 +150,28 @@ __device__ __forceinline__ void resolve(Scalars& c) {
 // Products and sums of the moments are rounded one by one (no fused multiply-add), so that the 8-bit codes follow from
 // elementary operations; the parameter's update uses the hardware's approximate square root and reciprocal (a few units
 // in the last place of an update that is itself a small part of the parameter).
-__device__ __forceinline__ void update(const Scalars& c, float& p, float g, float& m, float& v) {
-    g = __fmul_rn(g, c.scale);
-    m = __fadd_rn(__fmul_rn(m, c.b1), __fmul_rn(g, c.omb1));
-    v = __fadd_rn(__fmul_rn(v, c.b2), __fmul_rn(__fmul_rn(g, g), c.omb2));
-    float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
-    r = fmaf(r, c.inv, c.eps);   // between 2^-75 (or 0) and 2^65: its reciprocal needs no care for subnormals
-    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r));
-    p = fmaf(p, c.decay, -(c.step * m) * r);
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ void update2(const Scalars& c, float2& p, float2 g, float2& m, float2& v) {
+    // a b + c as (a b) * one + c, one = 1 only at run time: a packed product and a packed sum would be joined to one rounding
+    const float2 one = both(c.one);
+    g = __fmul2_rn(g, both(c.scale));
+    m = __ffma2_rn(__fmul2_rn(m, both(c.b1)), one, __fmul2_rn(g, both(c.omb1)));
+    v = __ffma2_rn(__fmul2_rn(v, both(c.b2)), one, __fmul2_rn(__fmul2_rn(g, g), both(c.omb2)));
+    float2 r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
+    r = __ffma2_rn(r, both(c.inv), both(c.eps));   // between 2^-75 (or 0) and 2^65: its reciprocal needs no care for subnormals
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r.x));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r.y));
+    p = __ffma2_rn(__fmul2_rn(m, both(-c.step)), r, __fmul2_rn(p, both(c.decay)));
+}
+__device__ __forceinline__ void update(const Scalars& c, float (&p)[kVec], const float (&g)[kVec], float (&m)[kVec], float (&v)[kVec]) {
+#pragma unroll
+    for (int i = 0; i < kVec; i += 2) {   // two elements to an instruction
+        float2 p2 = make_float2(p[i], p[i + 1]), m2 = make_float2(m[i], m[i + 1]), v2 = make_float2(v[i], v[i + 1]);
+        update2(c, p2, make_float2(g[i], g[i + 1]), m2, v2);
+        p[i] = p2.x; p[i + 1] = p2.y; m[i] = m2.x; m[i + 1] = m2.y; v[i] = v2.x; v[i + 1] = v2.y;
+    }
 }
 
 // ---- 8-bit codes
@@ -188,9 +212,9 @@ struct State8 {
 };
 
 // Where the 16 random bits of each value come from: the low half of word i is m's, the high half v's.
-struct Noise {          // two neighbouring elements share a 64-bit draw
+struct Noise {          // two neighbouring elements share a 64-bit draw; i counts the lane's elements
     uint64_t key, pair; // pair: half the index of the lane's first element (which is even)
-    __device__ __forceinline__ uint64_t operator()(int i) const { return draw64(key, pair + (uint64_t)(i / 2)); }
+    __device__ __forceinline__ uint64_t operator()(int i) const { return draw64(key, pair + (uint64_t)(i / 4 * 64 + i % 4 / 2)); }
 };
 struct Nearest {        // half a grid step
     __device__ __forceinline__ uint64_t operator()(int) const { return 0x8000800080008000ull; }
@@ -264,16 +288,21 @@ __device__ __forceinline__ void encode(const State8& s, long long at, int lane, 
         encode_slow(am, av, rnd, out);
         wm[0] = out[0]; wm[1] = out[1]; wv[0] = out[2]; wv[1] = out[3]; bm = out[4]; bv = out[5];
     }
-    *reinterpret_cast<uint2*>(s.m + at + lane * kVec) = make_uint2(wm[0], wm[1]);
-    *reinterpret_cast<uint2*>(s.v + at + lane * kVec) = make_uint2(wv[0], wv[1]);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        *reinterpret_cast<uint32_t*>(s.m + at + 128 * h + lane * 4) = wm[h];
+        *reinterpret_cast<uint32_t*>(s.v + at + 128 * h + lane * 4) = wv[h];
+    }
     if (lane == 0) { s.mb[at / kBlock] = (uint16_t)bm; s.vb[at / kBlock] = (uint16_t)bv; }
 }
 // The lane's eight values of one block: loaded (fetch) and decoded later (values), so that all loads are in flight first.
 struct Codes { uint2 m, v; uint32_t bm, bv; };
 __device__ __forceinline__ Codes fetch(const State8& s, long long at, int lane) {
     Codes c;
-    c.m = *reinterpret_cast<const uint2*>(s.m + at + lane * kVec);
-    c.v = *reinterpret_cast<const uint2*>(s.v + at + lane * kVec);
+    c.m.x = *reinterpret_cast<const uint32_t*>(s.m + at + lane * 4);
+    c.m.y = *reinterpret_cast<const uint32_t*>(s.m + at + 128 + lane * 4);
+    c.v.x = *reinterpret_cast<const uint32_t*>(s.v + at + lane * 4);
+    c.v.y = *reinterpret_cast<const uint32_t*>(s.v + at + 128 + lane * 4);
     c.bm = s.mb[at / kBlock]; c.bv = s.vb[at / kBlock];
     return c;
 }
@@ -301,36 +330,34 @@ __device__ __forceinline__ void values(const Codes& c, float (&m)[kVec], float (
     }
 }
 
-// ---- the kernels: a warp takes one block of 256 elements, a lane eight in a row
+// ---- the kernels: a warp takes one block of 256 elements, a lane two quads of it
 template <int BITS, class P, class G, int N>
 __device__ __forceinline__ void step_block(const StepArgs<N>& a, const Scalars& c, const Chunk& ch, void* p, const void* g, int lane, int block) {
-    const int n = min(kVec, max(0, ch.n - block - lane * kVec));   // this lane's elements
-    const long long at = ch.start + block + lane * kVec;
+    const int left = ch.n - block - lane * 4;   // elements from this lane's first one to the end
+    const long long at = ch.start + block + lane * 4;
     const long long st = ch.state + block;
     float pv[kVec], gv[kVec], m[kVec], v[kVec];
-    load8<P>(p, ch.param_type, at, n, pv);
-    load8<G>(g, ch.grad_type, at, n, gv);
+    load8<P>(p, ch.param_type, at, left, pv);
+    load8<G>(g, ch.grad_type, at, left, gv);
     if constexpr (BITS == 32) {
-        float* sm = static_cast<float*>(a.state) + st + lane * kVec;
+        float* sm = static_cast<float*>(a.state) + st + lane * 4;
         float* sv = sm + a.total;
-        load8(sm, kVec, m);
-        load8(sv, kVec, v);
-#pragma unroll
-        for (int i = 0; i < kVec; i++) update(c, pv[i], gv[i], m[i], v[i]);
-        store8(sm, n, m);
-        store8(sv, n, v);
-        store8<P>(p, ch.param_type, at, n, pv);
+        load8(sm, kBlock, m);
+        load8(sv, kBlock, v);
+        update(c, pv, gv, m, v);
+        store8(sm, left, m);
+        store8(sv, left, v);
+        store8<P>(p, ch.param_type, at, left, pv);
     } else {
         const State8 s(a.state, a.total);
         const Codes codes = fetch(s, st, lane);
         values(codes, m, v);
-#pragma unroll
-        for (int i = 0; i < kVec; i++) update(c, pv[i], gv[i], m[i], v[i]);
-        store8<P>(p, ch.param_type, at, n, pv);
-        if (n < kVec) {
+        update(c, pv, gv, m, v);
+        store8<P>(p, ch.param_type, at, left, pv);
+        if (left < 132) {
 #pragma unroll
             for (int i = 0; i < kVec; i++)
-                if (i >= n) m[i] = v[i] = 0.0f;   // behind the tensor's end
+                if (i / 4 * 128 + i % 4 >= left) m[i] = v[i] = 0.0f;   // behind the tensor's end
         }
         encode(s, st, lane, m, v, Noise{stream_key(c.seed, kStreamAdamW, c.it, (uint32_t)ch.tensor), (uint64_t)at >> 1});
     }
@@ -358,16 +385,16 @@ __global__ void __launch_bounds__(256) k_adamw_get(const State8 s, long long tot
     if (at >= total) return;
     float m[kVec], v[kVec];
     values(fetch(s, at, lane), m, v);
-    store8(fm + at + lane * kVec, kVec, m);
-    store8(fv + at + lane * kVec, kVec, v);
+    store8(fm + at + lane * 4, kBlock, m);
+    store8(fv + at + lane * 4, kBlock, v);
 }
 __global__ void __launch_bounds__(256) k_adamw_set(const State8 s, long long total, const float* __restrict__ fm, const float* __restrict__ fv) {
     const int lane = threadIdx.x & 31;
     const long long at = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * kBlock;
     if (at >= total) return;
     float m[kVec], v[kVec];
-    load8(fm + at + lane * kVec, kVec, m);
-    load8(fv + at + lane * kVec, kVec, v);
+    load8(fm + at + lane * 4, kBlock, m);
+    load8(fv + at + lane * 4, kBlock, v);
     encode(s, at, lane, m, v, Nearest{});
 }
 
@@ -514,7 +541,7 @@ int ntcb_adamw_step(const ntcb_adamw* a, void* const* params, const void* const*
     c.log_beta1 = std::log(args->beta1); c.log_beta2 = std::log(args->beta2);
     c.b1 = (float)args->beta1; c.omb1 = (float)(1.0 - args->beta1);
     c.b2 = (float)args->beta2; c.omb2 = (float)(1.0 - args->beta2);
-    c.eps = (float)args->eps; c.scale = (float)args->grad_scale;
+    c.eps = (float)args->eps; c.scale = (float)args->grad_scale; c.one = 1.0f;
     if (!args->it_dev) {
         c.step = (float)(args->lr / (1.0 - std::pow(args->beta1, (double)args->it)));
         c.inv = (float)(1.0 / std::sqrt(1.0 - std::pow(args->beta2, (double)args->it)));
