@@ -20,5 +20,6 @@ __all__ += list(_TORCH_NAMES)
 def __getattr__(name):
     if name in _TORCH_NAMES:
         from importlib import import_module
-        return getattr(import_module("." + _TORCH_NAMES[name], __name__), name)
+        value = globals()[name] = getattr(import_module("." + _TORCH_NAMES[name], __name__), name)
+        return value
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

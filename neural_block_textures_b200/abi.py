@@ -203,14 +203,14 @@ SIGNATURES = {
     "ntcb_p2p_release": (None, [_vp]),
     "ntcb_p2p_set_poll_limit": (None, [_vp, C.c_uint]),
     "ntcb_p2p_barrier": (C.c_int, [_vp, C.c_uint]),
-    "ntcb_symbol_logprobs": (C.c_int, [C.POINTER(SymbolDesc), _vp, _vp, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, C.c_char_p, C.c_size_t]),
-    "ntcb_symbol_logprobs_grad": (C.c_int, [C.POINTER(SymbolDesc), _vp, _vp, _vp, _vp, _vp, C.c_longlong, _vp, C.c_longlong, _vp, C.c_longlong,
+    "ntcb_symbol_logprobs": (C.c_int, [_vp, _vp, _vp, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, C.c_char_p, C.c_size_t]),
+    "ntcb_symbol_logprobs_grad": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, C.c_longlong, _vp, C.c_longlong, _vp, C.c_longlong,
                                             _vp, C.c_char_p, C.c_size_t]),
     "ntcb_adamw_create": (_vp, [C.c_int, C.c_int, C.POINTER(C.c_longlong), _ip, _ip, C.c_int, C.c_char_p, C.c_size_t]),
     "ntcb_adamw_destroy": (None, [_vp]),
     "ntcb_adamw_state_bytes": (C.c_size_t, [_vp]),
     "ntcb_adamw_offset": (C.c_longlong, [_vp, C.c_int]),
-    "ntcb_adamw_step": (C.c_int, [_vp, _vp, _vp, _vp, C.POINTER(AdamWArgs), _vp, C.c_char_p, C.c_size_t]),
+    "ntcb_adamw_step": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, C.c_char_p, C.c_size_t]),
     "ntcb_adamw_get_moments": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_char_p, C.c_size_t]),
     "ntcb_adamw_set_moments": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_char_p, C.c_size_t]),
 }

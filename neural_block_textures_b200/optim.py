@@ -18,7 +18,10 @@ from array import array
 import torch
 
 from . import abi
-from .symbols import DTYPES, _call
+from .symbols import DTYPES, _call, _raw_stream
+
+_T = torch.Tensor
+_dtype_of = _T.dtype.__get__
 
 
 class AdamW:
@@ -53,12 +56,14 @@ class AdamW:
         self.device = self.params[0].device
         self.state_bits, self.betas, self.eps, self.weight_decay, self.seed = state_bits, tuple(betas), eps, weight_decay, seed
         n = len(self.params)
-        self._shape = [(p.numel(), p.dtype, grad_dtype or p.dtype) for p in self.params]
+        self._index = self.device.index
+        self._sizes = [p.numel() for p in self.params]
+        self._grad_dtypes = [grad_dtype or p.dtype for p in self.params]
         self.lib = abi.load_library()
         why = C.create_string_buffer(256)
         self.h = self.lib.ntcb_adamw_create(
-            self.device.index, n, (C.c_longlong * n)(*[s[0] for s in self._shape]), (C.c_int * n)(*[DTYPES[s[1]] for s in self._shape]),
-            (C.c_int * n)(*[DTYPES[s[2]] for s in self._shape]), state_bits, why, 256)
+            self.device.index, n, (C.c_longlong * n)(*self._sizes), (C.c_int * n)(*[DTYPES[p.dtype] for p in self.params]),
+            (C.c_int * n)(*[DTYPES[t] for t in self._grad_dtypes]), state_bits, why, 256)
         if not self.h:
             raise RuntimeError("AdamW: " + why.value.decode())
         self.offsets = [int(self.lib.ntcb_adamw_offset(self.h, i)) for i in range(n + 1)]   # elements; the last is the total
@@ -87,6 +92,16 @@ class AdamW:
             raise ValueError(f"AdamW.step: {name} as a tensor must be one {dtype} on {self.device}")
         return None, x.data_ptr()
 
+    def _addresses(self, params, grads, live) -> tuple[array, array]:
+        """The tensors' addresses, after checking them against the plan (`live`: which of its tensors; None: all)."""
+        sizes, dtypes = (self._sizes, self._grad_dtypes) if live is None else ([self._sizes[i] for i in live], [self._grad_dtypes[i] for i in live])
+        if list(map(_T.numel, params)) != sizes or not all(map(_T.is_contiguous, params)):
+            raise ValueError("AdamW.step: a parameter's size or layout has changed")
+        if (list(map(_T.numel, grads)) != sizes or list(map(_dtype_of, grads)) != dtypes or not all(map(_T.is_contiguous, grads))
+                or not set(map(_T.get_device, grads)) <= {self._index}):
+            raise ValueError("AdamW.step: a gradient must be contiguous, on the parameters' device and of its parameter's size and the plan's type")
+        return array("Q", map(_T.data_ptr, params)), array("Q", map(_T.data_ptr, grads))
+
     def step(self, it, lr, grads=None, grad_scale=1.0) -> None:
         """Step number `it` (from 1) at learning rate `lr` with the gradients `grads` (default: each p.grad) times
         grad_scale; a None gradient leaves its tensor and moments alone. it, lr and grad_scale may be device tensors
@@ -96,26 +111,21 @@ class AdamW:
             grads = [p.grad for p in self.params]
         if len(grads) != len(self.params):
             raise ValueError(f"AdamW.step: {len(self.params)} gradients are needed, not {len(grads)}")
-        device = self.device
-        pp, gg = array("Q"), array("Q")
-        for p, g, (n, dtype, grad_dtype) in zip(self.params, grads, self._shape):
-            if g is None:
-                pp.append(0)
-                gg.append(0)
-                continue
-            if p.numel() != n or p.dtype is not dtype or p.device != device or not p.is_contiguous():
-                raise ValueError("AdamW.step: a parameter's size, type, device or layout has changed")
-            if g.numel() != n or g.dtype is not grad_dtype or g.device != device or not g.is_contiguous():
-                raise ValueError(f"AdamW.step: a gradient must be a contiguous {grad_dtype} tensor of {n} elements on {device}")
-            pp.append(p.data_ptr())
-            gg.append(g.data_ptr())
+        params, index = self.params, self._index
+        try:
+            pp, gg = self._addresses(params, grads, None)
+        except TypeError:   # something in grads is no tensor: None is allowed
+            live = [i for i, g in enumerate(grads) if g is not None]
+            pp, gg = array("Q", bytes(8 * len(params))), array("Q", bytes(8 * len(params)))
+            for i, p, g in zip(live, *self._addresses([params[i] for i in live], [grads[i] for i in live], live)):
+                pp[i], gg[i] = p, g
         it, it_dev = self._scalar(it, torch.int64, "it")
         lr, lr_dev = self._scalar(lr, torch.float32, "lr")
         scale, scale_dev = self._scalar(grad_scale, torch.float32, "grad_scale")
         args = abi.AdamWArgs(0.0 if lr is None else lr, self.betas[0], self.betas[1], self.eps, self.weight_decay,
                              1.0 if scale is None else scale, 0 if it is None else it, self.seed & (1 << 64) - 1, it_dev, lr_dev, scale_dev)
         _call(self.lib.ntcb_adamw_step, "AdamW.step", self.h, pp.buffer_info()[0], gg.buffer_info()[0], self.state.data_ptr(),
-              C.byref(args), torch.cuda.current_stream(device).cuda_stream)
+              C.byref(args), _raw_stream(index))
 
     def moments_flat(self) -> tuple[torch.Tensor, torch.Tensor]:
         """(m, v) as flat float32 tensors, tensor i at offsets[i]: the state itself with 32 bits, the values that the
@@ -128,7 +138,7 @@ class AdamW:
         m = torch.empty(total, dtype=torch.float32, device=self.device)
         v = torch.empty_like(m)
         _call(self.lib.ntcb_adamw_get_moments, "AdamW.moments", self.h, self.state.data_ptr(), m.data_ptr(), v.data_ptr(),
-              torch.cuda.current_stream(self.device).cuda_stream)
+              _raw_stream(self._index))
         return m, v
 
     def moments(self) -> tuple[list[torch.Tensor], list[torch.Tensor]]:
@@ -140,21 +150,21 @@ class AdamW:
         self._open()
         flat = []
         for name, xs in (("m", list(m)), ("v", list(v))):
-            if len(xs) != len(self.params) or any(x.numel() != s[0] for x, s in zip(xs, self._shape)):
+            if len(xs) != len(self.params) or any(x.numel() != n for x, n in zip(xs, self._sizes)):
                 raise ValueError(f"AdamW.set_moments: {name} must have one tensor of each parameter's size")
             f = torch.zeros(self.offsets[-1], dtype=torch.float32, device=self.device)
             for o, x in zip(self.offsets, xs):
                 f[o:o + x.numel()].copy_(x.reshape(-1))
             flat.append(f)
         _call(self.lib.ntcb_adamw_set_moments, "AdamW.set_moments", self.h, flat[0].data_ptr(), flat[1].data_ptr(),
-              self.state.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream)
+              self.state.data_ptr(), _raw_stream(self._index))
 
     def state_dict(self) -> dict:
         """The state (a copy) with what it was laid out for."""
-        return {"state_bits": self.state_bits, "sizes": [s[0] for s in self._shape], "state": self.state.clone()}
+        return {"state_bits": self.state_bits, "sizes": list(self._sizes), "state": self.state.clone()}
 
     def load_state_dict(self, d: dict) -> None:
-        if d["state_bits"] != self.state_bits or list(d["sizes"]) != [s[0] for s in self._shape]:
+        if d["state_bits"] != self.state_bits or list(d["sizes"]) != self._sizes:
             raise ValueError("AdamW.load_state_dict: the state is of another layout")
         if d["state"].dtype != torch.uint8 or d["state"].numel() != self.state.numel():
             raise ValueError("AdamW.load_state_dict: the state has another size")

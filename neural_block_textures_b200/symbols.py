@@ -11,6 +11,7 @@ Calls run on torch's current stream of the logits' device, without synchronising
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import NamedTuple
 
 import torch
@@ -29,25 +30,33 @@ class SymbolLogprobs(NamedTuple):
     top_logp: torch.Tensor   # [n, topk] float32; -inf there
 
 
-def _desc(logits: torch.Tensor, symbols: torch.Tensor, name: str) -> abi.SymbolDesc:
+_pack_desc = struct.Struct("4i4q").pack   # ntcb_symbol_desc
+# torch's current stream of a device as an address; the public call makes an object for it (2 us of a 12 us call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _desc(logits: torch.Tensor, symbols: torch.Tensor, name: str) -> tuple[bytes, int, int, int]:
+    """(ntcb_symbol_desc, rows, vocab, device index) of checked arguments."""
     if not isinstance(logits, torch.Tensor) or not isinstance(symbols, torch.Tensor):
         raise TypeError(f"{name}: logits and symbols must be torch tensors")
-    if logits.dtype not in DTYPES:
+    dtype, symbol_type = DTYPES.get(logits.dtype), SYMBOL_TYPES.get(symbols.dtype)
+    if dtype is None:
         raise TypeError(f"{name}: logits must be float32, float16 or bfloat16, not {logits.dtype}")
-    if symbols.dtype not in SYMBOL_TYPES:
+    if symbol_type is None:
         raise TypeError(f"{name}: symbols must be uint8, int16, int32 or int64, not {symbols.dtype}")
-    if logits.dim() != 2 or logits.shape[1] < 1:
-        raise ValueError(f"{name}: logits must be [rows, vocab] with vocab >= 1, not {tuple(logits.shape)}")
-    n, v = logits.shape
+    shape = logits.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"{name}: logits must be [rows, vocab] with vocab >= 1, not {tuple(shape)}")
+    n, v = shape
     if symbols.shape != (n,):
         raise ValueError(f"{name}: symbols must be [{n}], not {tuple(symbols.shape)}")
-    if not logits.is_cuda or symbols.device != logits.device:
+    device = logits.get_device()
+    if device < 0 or symbols.get_device() != device:
         raise ValueError(f"{name}: logits and symbols must be on one CUDA device")
-    row_stride = logits.stride(0) if n > 1 else v
-    if v > 1 and logits.stride(1) != 1:
+    row_stride, stride = logits.stride()
+    if v > 1 and stride != 1:
         raise ValueError(f"{name}: a row's logits must be contiguous")
-    return abi.SymbolDesc(logits.device.index, DTYPES[logits.dtype], SYMBOL_TYPES[symbols.dtype], 0, n, v, row_stride,
-                          symbols.stride(0))
+    return _pack_desc(device, dtype, symbol_type, 0, n, v, row_stride if n > 1 else v, symbols.stride(0)), n, v, device
 
 
 def _call(fn, name: str, *args) -> None:
@@ -56,27 +65,25 @@ def _call(fn, name: str, *args) -> None:
         raise RuntimeError(f"{name}: {why.value.decode()}")
 
 
-def _per_row(x: torch.Tensor, n: int, device: torch.device, name: str) -> torch.Tensor:
-    if x.dtype != torch.float32 or x.shape != (n,) or x.device != device:
-        raise ValueError(f"symbol_logprobs_grad: {name} must be a float32 tensor of [{n}] on {device}")
+def _per_row(x: torch.Tensor, n: int, device: int, name: str) -> torch.Tensor:
+    if x.dtype is not torch.float32 or x.shape != (n,) or x.get_device() != device:
+        raise ValueError(f"symbol_logprobs_grad: {name} must be a float32 tensor of [{n}] on the logits' device")
     return x
 
 
 def symbol_logprobs(logits: torch.Tensor, symbols: torch.Tensor, topk: int = 0) -> SymbolLogprobs:
     """Log probabilities of `symbols` [n] under `logits` [n, V] with the rows' entropy, log-sum-exp and `topk` (0 .. 32,
     at most V) likeliest symbols, in one pass over the logits. Rows may be strided; a row's logits are contiguous."""
-    d = _desc(logits, symbols, "symbol_logprobs")
-    n, v = d.rows, d.vocab
+    d, n, v, device = _desc(logits, symbols, "symbol_logprobs")
     if not 0 <= topk <= min(abi.MAX_TOPK, v):
         raise ValueError(f"symbol_logprobs: topk must be 0 .. {min(abi.MAX_TOPK, v)} here, not {topk}")
-    dev = logits.device
-    out = torch.empty(3, n, dtype=torch.float32, device=dev)
-    ids = torch.empty(n, topk, dtype=torch.int32, device=dev)
-    top = torch.empty(n, topk, dtype=torch.float32, device=dev)
+    # one allocation: a small call is mostly host work (2 us an allocation)
+    out = torch.empty(n * (3 + 2 * topk), dtype=torch.float32, device=logits.device)
+    logp, entropy, lse, top, ids = out.split_with_sizes((n, n, n, n * topk, n * topk))
     p = out.data_ptr()
-    _call(abi.load_library().ntcb_symbol_logprobs, "symbol_logprobs", C.byref(d), logits.data_ptr(), symbols.data_ptr(), topk,
-          p, p + 4 * n, p + 8 * n, ids.data_ptr(), top.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
-    return SymbolLogprobs(out[0], out[1], out[2], ids, top)
+    _call(abi.load_library().ntcb_symbol_logprobs, "symbol_logprobs", d, logits.data_ptr(), symbols.data_ptr(), topk,
+          p, p + 4 * n, p + 8 * n, p + 4 * n * (3 + topk), p + 12 * n, _raw_stream(device))
+    return SymbolLogprobs(logp, entropy, lse, ids.view(torch.int32).view(n, topk), top.view(n, topk))
 
 
 def symbol_logprobs_grad(logits: torch.Tensor, symbols: torch.Tensor, lse: torch.Tensor, entropy: torch.Tensor | None,
@@ -85,23 +92,22 @@ def symbol_logprobs_grad(logits: torch.Tensor, symbols: torch.Tensor, lse: torch
     """The gradient of sum(dlogp * logp + dentropy * entropy) for the logits, in their type, from the forward pass's lse
     and entropy. dlogp / dentropy: [n] float32 (any stride, so an expanded scalar too) or a number for every row.
     out: where to write it, of the logits' shape and type; the logits themselves are allowed."""
-    d = _desc(logits, symbols, "symbol_logprobs_grad")
-    n, v = d.rows, d.vocab
+    d, n, v, device = _desc(logits, symbols, "symbol_logprobs_grad")
     dev = logits.device
     if not isinstance(dlogp, torch.Tensor):
         dlogp = torch.full((1,), float(dlogp), device=dev).expand(n)
     if dentropy is not None and not isinstance(dentropy, torch.Tensor):
         dentropy = torch.full((1,), float(dentropy), device=dev).expand(n)
-    _per_row(lse, n, dev, "lse")
-    _per_row(dlogp, n, dev, "dlogp")
+    _per_row(lse, n, device, "lse")
+    _per_row(dlogp, n, device, "dlogp")
     if dentropy is not None:
         if entropy is None:
             raise ValueError("symbol_logprobs_grad: dentropy needs the forward pass's entropy")
-        _per_row(entropy, n, dev, "entropy")
-        _per_row(dentropy, n, dev, "dentropy")
+        _per_row(entropy, n, device, "entropy")
+        _per_row(dentropy, n, device, "dentropy")
         entropy = entropy.contiguous()
     if out is None:
-        out = torch.empty(n, v, dtype=logits.dtype, device=dev)
+        out = logits.new_empty((n, v))
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev:
         raise ValueError("symbol_logprobs_grad: out must have the logits' shape, type and device")
     elif (v > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < v):
@@ -109,8 +115,8 @@ def symbol_logprobs_grad(logits: torch.Tensor, symbols: torch.Tensor, lse: torch
     elif out.data_ptr() == logits.data_ptr() and n > 1 and out.stride(0) != logits.stride(0):
         raise ValueError("symbol_logprobs_grad: out over the logits needs their row stride")
     lse = lse.contiguous()
-    _call(abi.load_library().ntcb_symbol_logprobs_grad, "symbol_logprobs_grad", C.byref(d), logits.data_ptr(), symbols.data_ptr(),
+    _call(abi.load_library().ntcb_symbol_logprobs_grad, "symbol_logprobs_grad", d, logits.data_ptr(), symbols.data_ptr(),
           lse.data_ptr(), entropy.data_ptr() if dentropy is not None else None, dlogp.data_ptr(), dlogp.stride(0),
           dentropy.data_ptr() if dentropy is not None else None, dentropy.stride(0) if dentropy is not None else 0, out.data_ptr(),
-          out.stride(0) if n > 1 else v, torch.cuda.current_stream(dev).cuda_stream)
+          out.stride(0) if n > 1 else v, _raw_stream(device))
     return out
