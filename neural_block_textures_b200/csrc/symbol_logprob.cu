@@ -205,13 +205,16 @@ __device__ __forceinline__ RowOut finish_row(const Sums& q) {
     o.entropy = o.empty ? 0.0f : o.log_s - q.u / q.s;
     return o;
 }
-// The row's scalars, by one thread; t is its symbol, fetched with the row (the logit itself is in L1 or L2 by then).
-template <class T>
-__device__ __forceinline__ void write_row(const RowArgs& a, long long r, const T* row, long long t, const RowOut& o) {
-    const float xt = t >= 0 && t < a.V ? to_f32(row[t]) : NAN;
+// The row's scalars, by one thread; t is its symbol (fetched with the row), xt the symbol's logit, NaN where there is none.
+__device__ __forceinline__ void write_row(const RowArgs& a, long long r, float xt, long long t, const RowOut& o) {
     a.logp[r] = t < 0 ? 0.0f : o.bad ? NAN : o.empty ? (t < a.V ? kNegInf : NAN) : (xt - o.m) - o.log_s;
     a.entropy[r] = o.bad ? NAN : o.entropy;
     a.lse[r] = o.bad ? NAN : o.lse;
+}
+// The logit is in L1 or L2 by the time the row is summed up.
+template <class T>
+__device__ __forceinline__ void write_row(const RowArgs& a, long long r, const T* row, long long t, const RowOut& o) {
+    write_row(a, r, t >= 0 && t < a.V ? to_f32(row[t]) : NAN, t, o);
 }
 
 // ------------------------------------------------------------------------------------------------------------- keys
@@ -381,7 +384,22 @@ __global__ void __launch_bounds__(256) k_logprobs_lanes(const RowArgs a) {
 #pragma unroll
     for (int o = G / 2; o; o >>= 1) q2 = __fadd2_rn(q2, make_float2(__shfl_xor_sync(kFull, q2.x, o), __shfl_xor_sync(kFull, q2.y, o)));
     const RowOut o = finish_row(sums_of(m, sc, q2.x, q2.y));
-    if (live && lane == 0) write_row(a, r, row, t, o);
+    if (live && lane == 0) {
+        if constexpr (G == 1 && E <= 8) {   // the logit is at hand
+            float xt = NAN;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                float x[N];
+                expand<T>(raw[c], x);
+#pragma unroll
+                for (int i = 0; i < N; i++)
+                    if (t >= 0 && t < V && c * N + i - shift == (int)t) xt = x[i];
+            }
+            write_row(a, r, xt, t, o);
+        } else {
+            write_row(a, r, row, t, o);
+        }
+    }
     if constexpr (L > 0) {
         K k[E];
 #pragma unroll
@@ -412,16 +430,21 @@ __global__ void __launch_bounds__(256) k_logprobs_lanes(const RowArgs a) {
 
 // ------------------------------------------------------------------------------------------------------- long rows
 
-// Shared memory of one row's threads (W warps): partial sums, the threads' best keys, candidate alternatives.
+// Shared memory of one row's threads (W warps).
+constexpr int kSlots = 16;     // parts of a thread's share of the row whose maxima are kept
+constexpr int kWork = 256;     // parts that are read again
+constexpr int kCand = 256;     // candidate alternatives
 template <class K, int W>
 struct LongShared {
-    static constexpr int kCand = W * 64;
     Sums part[W];
     Sums total;                 // this CTA's part of the row
-    K list[W][32];
     K top[32];                  // this CTA's alternatives
+    K lists[W][32];             // the cluster's
     K cand[kCand];
-    int count;
+    float most[W][32];          // the threads' maxima, sorted per warp
+    float slot[kSlots][32 * W];
+    unsigned short work[kWork];
+    int nwork, ncand;
 };
 
 __device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -442,10 +465,11 @@ __device__ __forceinline__ P peer_load(const P* p, unsigned rank) {   // a word 
 
 // One row per W warps (R rows in a CTA when W = 1), or per cluster of C CTAs of one row's part each. Vector c of the row
 // belongs to CTA c / per, and there to thread (c - first) % threads; a thread reads U vectors at a time.
-// Alternatives: each thread keeps its largest logit and the group of U vectors that holds it. The topk largest of the
-// threads' maxima are at least as large as the row's topk-th logit, and every logit that large lies with one of those
-// topk threads; so only their vectors are read again (from L2), by all threads together, and the few logits that pass
-// are sorted. What is far above that (a row of equal logits) is taken by one warp from a running list of 32.
+// Alternatives: the threads keep the maxima of up to kSlots parts of their share. The topk-th largest of the threads'
+// maxima bounds the row's topk-th logit from below, so only the parts whose maximum reaches it are read again (from L2,
+// by all threads together) and the few logits that reach it are sorted. Where many logits equal the bound (a row of one
+// value, a part masked by the lowest value) those above it are taken like this and the first equal ones in order; what
+// still is too much is gone through by one warp with a running list of 32.
 template <class T, class K, int W, int R>
 __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, int C) {
     constexpr int N = VEC<T>, kThreads = 32 * W, U = 4;
@@ -460,8 +484,12 @@ __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, i
     const int shift = row_shift(row), V = a.V;
     const int nvec = (V + shift + N - 1) / N;
     const int per = (nvec + C - 1) / C, first = min(nvec, (int)rank * per), end = min(nvec, first + per);
-    float m = kLowest, mine = kNegInf;   // the running maximum; this thread's largest logit (-inf: none)
-    int at = -1;                         // the first vector of the first group that holds it
+    const int rounds = (end - first + U * kThreads - 1) / (U * kThreads);
+    int lg = 0;   // rounds of a slot, as a power of two
+    while ((rounds - 1) >> lg >= kSlots) lg++;
+    float m = kLowest, mine = kNegInf;   // the running maximum; this slot's (-inf: no logit)
+    float most = kNegInf;                // this thread's largest logit
+    int round = 0;
     Scale sc(m);
     float2 s2 = make_float2(0.0f, 0.0f), u2 = s2;
     for (int c = first + tid; c < end; c += U * kThreads) {
@@ -475,7 +503,14 @@ __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, i
             expand<T>(raw[k], v);
             gm = fmaxf(gm, max_of(v));
         }
-        if (gm > mine) { mine = gm; at = c; }
+        if (a.topk) {
+            mine = fmaxf(mine, gm);
+            if (((++round) & ((1 << lg) - 1)) == 0) {
+                sh.slot[(round - 1) >> lg][tid] = mine;
+                most = fmaxf(most, mine);
+                mine = kNegInf;
+            }
+        }
         if (gm > m) {   // y of what is summed so far moves by the difference of the b
             const Scale to(gm);
             const float y = max_nan(to.b - sc.b, kYLow), e = exp2_of(y);
@@ -498,74 +533,101 @@ __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, i
         q = join(q, p);
     }
     if (lane == 0) sh.part[warp] = q;
-    if (tid == 0) sh.count = 0;
+    const int slots = (rounds + (1 << lg) - 1) >> lg;
     if (a.topk) {
-        K k = 0;
-        if (at >= 0) {
-#pragma unroll
-            for (int g = U - 1; g >= 0; g--) {
-                const int c = at + g * kThreads;
-                float v[N];
-                expand<T>(load_vec<true>(row, c < end ? c * N - shift : V, V), v);
-#pragma unroll
-                for (int i = N - 1; i >= 0; i--)
-                    if (v[i] == mine) k = key_of<T, K>(v[i], c * N + i - shift);
-            }
-        }
-        sh.list[warp][lane] = sort32(k, lane);
+        for (int k = round >> lg; k < slots; k++) { sh.slot[k][tid] = mine; most = fmaxf(most, mine); mine = kNegInf; }
+        if (tid == 0) sh.nwork = sh.ncand = 0;
+        sh.most[warp][lane] = sort32(most, lane);
     }
     sync();
     if (a.topk) {
 #pragma unroll
         for (int half = W / 2; half; half >>= 1) {
             if (warp < half) {
-                const K k = merge32(sh.list[warp][lane], sh.list[warp + half][lane], lane);
+                const float k = merge32(sh.most[warp][lane], sh.most[warp + half][lane], lane);
                 __syncwarp();
-                sh.list[warp][lane] = k;
+                sh.most[warp][lane] = k;
             }
             sync();
         }
-        const K least = sh.list[0][a.topk - 1];   // 0 when fewer threads than topk hold a logit
-        const int per_thread = (end - first + kThreads - 1) / kThreads, items = a.topk * per_thread;
-        const auto vector_of = [&](int item) {    // the item's vector, `end` for none
-            const K owner = item < items ? sh.list[0][item / per_thread] : 0;
-            if (!owner) return end;
-            return min(end, first + ((key_index(owner) + shift) / N - first) % kThreads + (item % per_thread) * kThreads);
-        };
-        for (int item = tid; item < items; item += kThreads) {
-            const int c = vector_of(item);
-            if (c == end) continue;
-            float v[N];
-            expand<T>(load_vec<true>(row, c * N - shift, V), v);
+        const float least = sh.most[0][a.topk - 1];   // -inf when fewer threads than topk hold a logit
+        // The logits that reach `least` (STRICT: that are above it) into cand; false where the lists do not hold them.
+        const auto collect = [&](auto strict) {
+            const auto reaches = [&](float v) { return strict ? v > least : v >= least && v > kNegInf; };
+            if (reaches(most))
+                for (int k = 0; k < slots; k++)
+                    if (reaches(sh.slot[k][tid])) {
+                        const int p = atomicAdd(&sh.nwork, 1);
+                        if (p < kWork) sh.work[p] = (unsigned short)(k * kThreads + tid);
+                    }
+            sync();
+            const int nwork = min(sh.nwork, kWork), each = U << lg;
+            for (int item = tid; item < nwork * each; item += kThreads) {
+                const int w = sh.work[item / each], k = item % each;
+                const int c = first + w % kThreads + ((w / kThreads) * each + k) * kThreads;
+                if (c >= end) continue;
+                float v[N];
+                expand<T>(load_vec<true>(row, c * N - shift, V), v);
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                if (!(v[i] > kNegInf)) continue;
-                const K k = key_of<T, K>(v[i], c * N + i - shift);
-                if (k >= least) {
-                    const int p = atomicAdd(&sh.count, 1);
-                    if (p < sh.kCand) sh.cand[p] = k;
-                }
+                for (int i = 0; i < N; i++)
+                    if (reaches(v[i])) {
+                        const int p = atomicAdd(&sh.ncand, 1);
+                        if (p < kCand) sh.cand[p] = key_of<T, K>(v[i], c * N + i - shift);
+                    }
             }
+            sync();
+            return sh.nwork <= kWork && sh.ncand <= kCand;
+        };
+        bool held = collect(std::false_type{}), ties = false;
+        if (!held) {   // many logits equal to `least`: only the first of them count, found in order below
+            sync();
+            if (tid == 0) sh.nwork = sh.ncand = 0;
+            sync();
+            held = collect(std::true_type{});
+            ties = true;
         }
-        sync();
         if (warp == 0) {
             K top = 0;
-            const int count = sh.count;
-            if (count <= sh.kCand) {
+            const int count = sh.ncand;
+            if (held) {
                 for (int i = 0; i < count; i += 32) {
                     const K k = sort32(i + lane < count ? sh.cand[i + lane] : (K)0, lane);
                     top = i ? merge32(top, k, lane) : k;
                 }
+                if (ties) {   // the first topk logits that equal `least`, already in order
+                    int found = 0;
+                    __syncwarp();
+                    for (int c0 = first; c0 < end && found < a.topk; c0 += 32) {
+                        const int c = c0 + lane;
+                        float v[N];
+                        expand<T>(load_vec<true>(row, c < end ? c * N - shift : V, V), v);
+                        int n = 0, before = 0;
+#pragma unroll
+                        for (int i = 0; i < N; i++) n += v[i] == least && v[i] > kNegInf;
+                        int all = n;
+#pragma unroll
+                        for (int o = 1; o < 32; o <<= 1) { const int b = __shfl_up_sync(kFull, all, o); if (lane >= o) all += b; }
+                        before = found + all - n;
+#pragma unroll
+                        for (int i = 0; i < N; i++)
+                            if (v[i] == least && v[i] > kNegInf) {
+                                if (before < 32) sh.cand[before] = key_of<T, K>(v[i], c * N + i - shift);
+                                before++;
+                            }
+                        found += __shfl_sync(kFull, all, 31);
+                    }
+                    __syncwarp();
+                    top = merge32(top, lane < found ? sh.cand[lane] : (K)0, lane);
+                }
             } else {
-                for (int i0 = 0; i0 < items; i0 += 32) {
-                    const int c = vector_of(i0 + lane);
+                for (int c0 = first; c0 < end; c0 += 32) {
+                    const int c = c0 + lane;
                     float v[N];
                     expand<T>(load_vec<true>(row, c < end ? c * N - shift : V, V), v);
 #pragma unroll
                     for (int i = 0; i < N; i++) {
-                        K k = v[i] > kNegInf ? key_of<T, K>(v[i], c * N + i - shift) : (K)0;
-                        const K last = __shfl_sync(kFull, top, 31);
-                        if (k < least || k < last) k = 0;
+                        K k = v[i] >= least && v[i] > kNegInf ? key_of<T, K>(v[i], c * N + i - shift) : (K)0;
+                        if (k < __shfl_sync(kFull, top, 31)) k = 0;
                         if (__any_sync(kFull, k != 0)) top = merge32(top, sort32(k, lane), lane);
                     }
                 }
@@ -585,14 +647,28 @@ __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, i
     if (W > 1 && C > 1) {
         sync();
         cluster_sync();
-        if (rank == 0 && warp == 0) {
-            K top = a.topk ? sh.top[lane] : (K)0;
-            for (int w = 1; w < C; w++) {
-                const Sums b{peer_load(&sh.total.m, w), peer_load(&sh.total.s, w), peer_load(&sh.total.u, w)};
-                q = join(q, b);
-                if (a.topk) top = merge32(top, peer_load(&sh.top[lane], w), lane);
+        if (rank == 0) {   // a warp for each CTA's list, then joined in pairs
+            if (warp < C && a.topk) sh.lists[warp][lane] = peer_load(&sh.top[lane], warp);
+            if (warp == 0) {
+                q = lane < C ? Sums{peer_load(&sh.total.m, lane), peer_load(&sh.total.s, lane), peer_load(&sh.total.u, lane)} : Sums{kLowest, 0.0f, 0.0f};
+#pragma unroll
+                for (int o = W / 2; o; o >>= 1) {
+                    const Sums b{__shfl_xor_sync(kFull, q.m, o), __shfl_xor_sync(kFull, q.s, o), __shfl_xor_sync(kFull, q.u, o)};
+                    q = join(q, b);
+                }
             }
-            sh.top[lane] = top;
+            if (a.topk) {
+                sync();
+                for (int half = C / 2; half; half >>= 1) {
+                    if (warp < half) {
+                        const K k = merge32(sh.lists[warp][lane], sh.lists[warp + half][lane], lane);
+                        __syncwarp();
+                        sh.lists[warp][lane] = k;
+                    }
+                    sync();
+                }
+                if (warp == 0) sh.top[lane] = sh.lists[0][lane];
+            }
         }
         cluster_sync();   // no CTA leaves while its shared memory is read
     }
@@ -688,11 +764,13 @@ __global__ void __launch_bounds__(256) k_logprobs_grad(const GradArgs a, int lg)
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-// The widest a row gets with its shift: rows that all start on a 16-byte boundary have none.
+// The widest a row gets with its shift. Starts lie a multiple of g elements past a 16-byte boundary, so no shift is
+// above VEC - g.
 template <class T>
 int row_span(const void* x, long long stride, int V) {
-    const bool even = reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride % VEC<T> == 0;
-    return even ? V : V + VEC<T> - 1;
+    const long long at = (long long)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)) | stride | VEC<T>;
+    const int g = (int)(at & -at);
+    return V + VEC<T> - g;
 }
 
 template <class T, int G, int E, int L>
@@ -753,6 +831,7 @@ cudaError_t launch_rows(const RowArgs& a, cudaStream_t s, int sms) {
     } else if (a.topk <= 8) {
         if (span <= N) { launch_lanes<T, 1, N, N>(a, s); done = true; }
         else if (span <= 8) { launch_lanes<T, 1, 8, 8>(a, s); done = true; }
+        else if (span <= 16) { launch_lanes<T, 1, 16, 8>(a, s); done = true; }
         else done = launch_lanes<T, sizeof(T) == 2 ? 32 : 16, 8>(a, span, s);
     } else {
         done = launch_lanes<T, 16, 16>(a, span, s);
