@@ -143,11 +143,23 @@ __device__ __forceinline__ void expand(const uint4& a, float (&v)[VEC<T>]) {
         else { __half2 h; memcpy(&h, &w[i], 4); const float2 f = __half22float2(h); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
     }
 }
-template <int N> __device__ __forceinline__ float max_of(const float (&v)[N]) {
-    float m = v[0];
+// The largest of a number of vectors' elements; NaN counts for nothing. 16-bit types in pairs.
+template <class T, int C>
+__device__ __forceinline__ float max_of(const uint4 (&a)[C]) {
+    if constexpr (sizeof(T) == 4) {
+        float m = kNegInf;
 #pragma unroll
-    for (int i = 1; i < N; i++) m = fmaxf(m, v[i]);
-    return m;
+        for (int c = 0; c < C; c++)
+            m = fmaxf(fmaxf(fmaxf(m, __uint_as_float(a[c].x)), fmaxf(__uint_as_float(a[c].y), __uint_as_float(a[c].z))), __uint_as_float(a[c].w));
+        return m;
+    } else {
+        typedef typename std::conditional<std::is_same_v<T, __half>, __half2, __nv_bfloat162>::type P;
+        const auto pair = [](uint32_t w) { P p; memcpy(&p, &w, 4); return p; };
+        P m = __hmax2(__hmax2(pair(a[0].x), pair(a[0].y)), __hmax2(pair(a[0].z), pair(a[0].w)));
+#pragma unroll
+        for (int c = 1; c < C; c++) m = __hmax2(m, __hmax2(__hmax2(pair(a[c].x), pair(a[c].y)), __hmax2(pair(a[c].z), pair(a[c].w))));
+        return fmaxf(fmaxf(to_f32(m.x), to_f32(m.y)), kNegInf);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------ a row's sums
@@ -363,13 +375,7 @@ __global__ void __launch_bounds__(256) k_logprobs_lanes(const RowArgs a) {
 #pragma unroll
     for (int c = 0; c < C; c++) raw[c] = load_vec<true>(row, (c * G + lane) * N - shift, V);
     const long long t = live && lane == 0 ? load_symbol(a.sym, a.sym_type, r * a.sym_stride) : -1;
-    float m = kLowest;   // a row of nothing but -inf keeps a finite maximum: y = -inf, e^d = 0
-#pragma unroll
-    for (int c = 0; c < C; c++) {
-        float x[N];
-        expand<T>(raw[c], x);
-        m = fmaxf(m, max_of(x));
-    }
+    float m = fmaxf(max_of<T>(raw), kLowest);   // a row of nothing but -inf keeps a finite maximum: y = -inf, e^d = 0
 #pragma unroll
     for (int o = G / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
     const Scale sc(m);
@@ -496,13 +502,7 @@ __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, i
         uint4 raw[U];
 #pragma unroll
         for (int k = 0; k < U; k++) raw[k] = load_vec<true>(row, c + k * kThreads < end ? (c + k * kThreads) * N - shift : V, V);
-        float gm = kNegInf;
-#pragma unroll
-        for (int k = 0; k < U; k++) {
-            float v[N];
-            expand<T>(raw[k], v);
-            gm = fmaxf(gm, max_of(v));
-        }
+        const float gm = max_of<T>(raw);
         if (a.topk) {
             mine = fmaxf(mine, gm);
             if (((++round) & ((1 << lg) - 1)) == 0) {
