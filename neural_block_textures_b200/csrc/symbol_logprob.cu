@@ -357,24 +357,80 @@ __device__ __forceinline__ K merge32(K a, K b, int lane) {
 
 // ------------------------------------------------------------------------------------------- rows in a few registers
 
-// G lanes hold one row of up to G * E elements (its shift counted in) in registers: the maximum is known before the
-// exponentials, so nothing is rescaled. Alternatives (L > 0): each lane sorts the L largest of its E keys (L = 1 for one
-// alternative, 8 for up to eight, E for more), and the row's next one is the largest of the lanes' first ones, which
-// its lane then drops.
-template <class T, int G, int E, int L>
-__global__ void __launch_bounds__(256) k_logprobs_lanes(const RowArgs a) {
-    constexpr int N = VEC<T>, C = E / N;
-    static_assert(E % N == 0, "whole vectors");
-    typedef typename std::conditional<sizeof(T) == 2, uint32_t, unsigned long long>::type K;
-    const long long r = (long long)blockIdx.x * (256 / G) + threadIdx.x / G;
-    const int lane = threadIdx.x % G;
-    const bool live = r < a.rows;
-    const T* row = static_cast<const T*>(a.x) + (live ? r : 0) * a.stride;
-    const int shift = row_shift(row), V = live ? a.V : 0;
-    uint4 raw[C];
+// The place of the first of a lane's elements that equals v (its vector's number c * G + lane times VEC, plus the
+// element's): -1 where none does. 16-bit types compare in pairs.
+template <class T, int G, int C>
+__device__ __forceinline__ int first_equal(const uint4 (&raw)[C], float v, int lane) {
+    constexpr int N = VEC<T>;
+    int at = -1;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int c = 0; c < C; c++) raw[c] = load_vec<true>(row, (c * G + lane) * N - shift, V);
-    const long long t = live && lane == 0 ? load_symbol(a.sym, a.sym_type, r * a.sym_stride) : -1;
+        for (int c = C - 1; c >= 0; c--) {
+            float x[N];
+            expand<T>(raw[c], x);
+#pragma unroll
+            for (int i = N - 1; i >= 0; i--)
+                if (x[i] == v) at = c * G * N + i;
+        }
+    } else {
+        typedef typename std::conditional<std::is_same_v<T, __half>, __half2, __nv_bfloat162>::type P;
+        P vv;
+        if constexpr (std::is_same_v<T, __half>) vv = __float2half2_rn(v); else vv = __float2bfloat162_rn(v);   // exact, or no logit
+        uint32_t hit = 0;   // bit w: the lower element of word w, bit 16 + w: the upper one
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                P p;
+                memcpy(&p, &w[i], 4);
+                hit |= __heq2_mask(p, vv) & (0x00010001u << (4 * c + i));
+            }
+        }
+        if (hit) {
+            const int lo = __ffs(hit & 0xffffu), hi = __ffs(hit >> 16);
+            const int e = min(lo ? 2 * (lo - 1) : 64, hi ? 2 * (hi - 1) + 1 : 64);
+            at = e / N * G * N + e % N;
+        }
+    }
+    return at < 0 ? -1 : at + lane * N;
+}
+
+// A row as a group of G lanes fetches it.
+template <class T, int C>
+struct RowIn {
+    uint4 raw[C];
+    const T* row;
+    long long r, t;
+    int shift, V;   // V = 0: no row
+};
+template <class T, int G, int C>
+__device__ __forceinline__ RowIn<T, C> fetch_row(const RowArgs& a, long long block) {
+    RowIn<T, C> f;
+    f.r = block * (256 / G) + threadIdx.x / G;
+    const int lane = threadIdx.x % G;
+    const bool live = f.r < a.rows;
+    f.row = static_cast<const T*>(a.x) + (live ? f.r : 0) * a.stride;
+    f.shift = row_shift(f.row);
+    f.V = live ? a.V : 0;
+#pragma unroll
+    for (int c = 0; c < C; c++) f.raw[c] = load_vec<true>(f.row, (c * G + lane) * VEC<T> - f.shift, f.V);
+    f.t = live && lane == 0 ? load_symbol(a.sym, a.sym_type, f.r * a.sym_stride) : -1;
+    return f;
+}
+
+// G lanes hold one row of up to G * E elements (its shift counted in) in registers: the maximum is known before the
+// exponentials, so nothing is rescaled. Alternatives (L > 0): each lane sorts the L largest of its E keys (8 for up to
+// eight alternatives, E for more), and the row's next one is the largest of the lanes' first ones, which its lane then
+// drops; a single alternative (L = 1) is the first logit that equals the maximum.
+template <class T, int G, int E, int L>
+__device__ __forceinline__ void rate_row(const RowArgs& a, const RowIn<T, E / VEC<T>>& f) {
+    constexpr int N = VEC<T>, C = E / N;
+    typedef typename std::conditional<sizeof(T) == 2, uint32_t, unsigned long long>::type K;
+    const auto& raw = f.raw;
+    const long long r = f.r, t = f.t;
+    const int lane = threadIdx.x % G, shift = f.shift, V = f.V;
+    const bool live = V > 0;
     float m = fmaxf(max_of<T>(raw), kLowest);   // a row of nothing but -inf keeps a finite maximum: y = -inf, e^d = 0
 #pragma unroll
     for (int o = G / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
@@ -403,10 +459,19 @@ __global__ void __launch_bounds__(256) k_logprobs_lanes(const RowArgs a) {
             }
             write_row(a, r, xt, t, o);
         } else {
-            write_row(a, r, row, t, o);
+            write_row(a, r, f.row, t, o);
         }
     }
-    if constexpr (L > 0) {
+    if constexpr (L == 1) {
+        int at = first_equal<T, G>(raw, m, lane);
+#pragma unroll
+        for (int w = G / 2; w; w >>= 1) at = (int)min((unsigned)at, (unsigned)__shfl_xor_sync(kFull, at, w));
+        if (live && lane == 0) {
+            const bool none = o.bad || o.empty;
+            a.top_ids[r] = none ? -1 : at - shift;
+            a.top_logp[r] = o.bad ? NAN : none ? kNegInf : -o.log_s;
+        }
+    } else if constexpr (L > 1) {
         K k[E];
 #pragma unroll
         for (int c = 0; c < C; c++) keys_of<T>(raw[c], (c * G + lane) * N, k + c * N);
@@ -432,6 +497,14 @@ __global__ void __launch_bounds__(256) k_logprobs_lanes(const RowArgs a) {
             }
         }
     }
+}
+
+// One group of rows to a CTA. (CTAs that stay and fetch the next rows ahead were slower on short rows: 17 against 15 us for
+// 2^20 rows of 4; the hardware's turnover of CTAs hides more.)
+template <class T, int G, int E, int L>
+__global__ void __launch_bounds__(256) k_logprobs_lanes(const RowArgs a) {
+    static_assert(E % VEC<T> == 0, "whole vectors");
+    rate_row<T, G, E, L>(a, fetch_row<T, G, E / VEC<T>>(a, blockIdx.x));
 }
 
 // ------------------------------------------------------------------------------------------------------- long rows
