@@ -432,6 +432,13 @@ cudaError_t launch_step(const ntcb_adamw* a, const Scalars& c, void* const* para
     return cudaGetLastError();
 }
 
+// Frees (a plan may be collected while some stream of the process is being captured) must not invalidate a capture.
+struct RelaxedCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 constexpr int kMaxPerLaunch = 1984;   // two addresses each: 31 KB of the 32 KB that a launch's arguments may take
 
 }  // namespace
@@ -496,6 +503,7 @@ ntcb_adamw* ntcb_adamw_create(int device, int ntensors, const long long* sizes, 
 
 void ntcb_adamw_destroy(ntcb_adamw* a) {
     if (!a) return;
+    ntcb::RelaxedCapture relaxed;
     if (a->chunks) cudaFree(a->chunks);
     delete a;
 }

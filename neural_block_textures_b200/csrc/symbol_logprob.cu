@@ -878,10 +878,14 @@ cudaError_t launch_long(const RowArgs& a, int C, cudaStream_t s) {
 
 template <class T, class K>
 cudaError_t launch_long(const RowArgs& a, int span, cudaStream_t s, int sms) {
+    // Warps to a row: eight, fewer as far as rows fill the GPU (24 warps an SM) or threads would not get two vectors. At
+    // 2048 x 65536 bf16 two took 55 us, eight 57; at 16384 x 4096 one took 30 us, eight 90.
+    // CTAs to a row: where rows are few, parts of 8192 logits or more on up to eight CTAs. 16 x 65536 took 5.2 us with eight,
+    // but 148 x 8192 8.6 us with four against 4.0 with one: clusters start slowly.
     int W = 8, C = 1;
-    while (W > 1 && (span < 64 * W * VEC<T> || a.rows * W / 2 >= 32ll * sms)) W /= 2;
+    while (W > 1 && (span < 64 * W * VEC<T> || a.rows * W / 2 >= 24ll * sms)) W /= 2;
     if (W == 8)
-        while (C < 8 && a.rows * C * 2 <= 4 * sms && a.V / (C * 2) >= 2048) C *= 2;
+        while (C < 8 && a.V / (C * 2) >= 8192 && a.rows * C * 2 <= 4 * sms) C *= 2;
     if (W == 1) return launch_long<T, K, 1, 4>(a, 1, s);
     if (W == 2) return launch_long<T, K, 2, 1>(a, 1, s);
     if (W == 4) return launch_long<T, K, 4, 1>(a, 1, s);
@@ -952,6 +956,16 @@ const char* check_desc(const ntcb_symbol_desc* d) {
 }
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 size_t dtype_size(int t) { return t == NTCB_F32 ? 4 : 2; }
+// Whether rows of V elements written at `out` (stride os) may share memory with the rows read at `in` (stride is): the same
+// rows, rows that lie between one another, or no common range at all.
+bool may_write(const void* in, long long is, const void* out, long long os, long long rows, long long V, size_t size) {
+    const long long a = (long long)(reinterpret_cast<uintptr_t>(in) / size), b = (long long)(reinterpret_cast<uintptr_t>(out) / size);
+    if (a + (rows - 1) * is + V <= b || b + (rows - 1) * os + V <= a) return true;
+    if (rows == 1) return a == b;
+    if (is != os) return false;
+    const long long off = ((b - a) % is + is) % is;
+    return a == b || (off >= V && off <= is - V);
+}
 size_t symbol_size(int t) { return t == NTCB_SYM_U8 ? 1 : t == NTCB_SYM_I16 ? 2 : t == NTCB_SYM_I32 ? 4 : 8; }
 
 }  // namespace
@@ -991,6 +1005,7 @@ extern "C" int ntcb_symbol_logprobs_grad(const ntcb_symbol_desc* d, const void* 
     if (!logits || !symbols || !lse || !dlogp || !dlogits || (dentropy && !entropy)) return refuse("null buffer");
     const size_t sz = dtype_size(d->dtype);
     if (!aligned(logits, sz) || !aligned(dlogits, sz) || !aligned(symbols, symbol_size(d->symbol_type))) return refuse("a buffer is not aligned to its type");
+    if (!may_write(logits, d->row_stride, dlogits, dlogits_stride, d->rows, d->vocab, sz)) return refuse("dlogits overlaps the logits without being them");
     DeviceScope scope(d->device, why, why_cap);
     if (!scope.ok) return 0;
     const GradArgs a{logits, symbols, lse, entropy, dlogp, dentropy, dlogits, d->rows, d->row_stride, d->symbol_stride, dlogits_stride,

@@ -8,7 +8,8 @@ the Adam that runs inside the trainer's own steps. With weight_decay 0 it is tha
         opt.step(it, lr)
 
 A step runs on torch's current stream of the parameters' device, without synchronising, and writes the parameters in
-place. In a captured CUDA graph the step number comes from the device: pass `it` as an int64 tensor and advance it there.
+place (autograd does not see that write). In a captured CUDA graph the step number comes from the device: pass `it` as an
+int64 tensor and advance it there.
 """
 from __future__ import annotations
 

@@ -91,7 +91,8 @@ def symbol_logprobs_grad(logits: torch.Tensor, symbols: torch.Tensor, lse: torch
                          out: torch.Tensor | None = None) -> torch.Tensor:
     """The gradient of sum(dlogp * logp + dentropy * entropy) for the logits, in their type, from the forward pass's lse
     and entropy. dlogp / dentropy: [n] float32 (any stride, so an expanded scalar too) or a number for every row.
-    out: where to write it, of the logits' shape and type; the logits themselves are allowed."""
+    out: where to write it, of the logits' shape and type; the logits themselves are allowed, memory
+    that overlaps them otherwise is refused."""
     d, n, v, device = _desc(logits, symbols, "symbol_logprobs_grad")
     dev = logits.device
     if not isinstance(dlogp, torch.Tensor):
@@ -112,8 +113,6 @@ def symbol_logprobs_grad(logits: torch.Tensor, symbols: torch.Tensor, lse: torch
         raise ValueError("symbol_logprobs_grad: out must have the logits' shape, type and device")
     elif (v > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < v):
         raise ValueError("symbol_logprobs_grad: out's rows must be contiguous and apart from one another")
-    elif out.data_ptr() == logits.data_ptr() and n > 1 and out.stride(0) != logits.stride(0):
-        raise ValueError("symbol_logprobs_grad: out over the logits needs their row stride")
     lse = lse.contiguous()
     _call(abi.load_library().ntcb_symbol_logprobs_grad, "symbol_logprobs_grad", d, logits.data_ptr(), symbols.data_ptr(),
           lse.data_ptr(), entropy.data_ptr() if dentropy is not None else None, dlogp.data_ptr(), dlogp.stride(0),

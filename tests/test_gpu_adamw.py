@@ -208,6 +208,35 @@ def test_none_gradients_and_p_grad(cuda_device):
     assert (p[0] - want).abs().max() < 1e-6 and opt.moments()[0][1].shape == (40, 5)
 
 
+def test_nothing_to_do(cuda_device):
+    opt = AdamW([torch.zeros(0, device="cuda"), torch.zeros(0, 3, device="cuda")], state_bits=8)
+    opt.step(1, 0.1, [torch.zeros(0, device="cuda"), None])
+    assert opt.moments()[0][1].shape == (0, 3) and opt.state.numel() == 0
+    p = torch.ones(5, device="cuda")
+    AdamW([p]).step(1, 0.1, [None])
+    assert (p == 1).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_two_plans_on_two_streams(bits, cuda_device):
+    sizes = [70001, 300]
+    sets = [tensors(sizes, "f32", s, 0.5) for s in (1, 2, 1, 2)]
+    grads = [tensors(sizes, "f32", s, 0.1) for s in (3, 4, 3, 4)]
+    for p, g in zip(sets[:2], grads[:2]):
+        opt = AdamW(p, state_bits=bits)
+        for it in (1, 2, 3):
+            opt.step(it, 0.01, g)
+    opts = [AdamW(p, state_bits=bits) for p in sets[2:]]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in opts]
+    for it in (1, 2, 3):
+        for st, opt, g in zip(streams, opts, grads[2:]):
+            with torch.cuda.stream(st):
+                opt.step(it, 0.01, g)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for x, y in zip(sets[:2], sets[2:]) for a, b in zip(x, y))
+
+
 def test_many_tensors_of_mixed_types(cuda_device):
     """More tensors than one launch's arguments hold, with several types in one call."""
     sizes = [(i * 37) % 600 for i in range(4100)]

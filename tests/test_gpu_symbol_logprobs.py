@@ -296,6 +296,70 @@ def test_streams_and_graphs(n, v, cuda_device):
     assert all(torch.equal(a, b) for a, b in zip(r, fresh))
 
 
+def test_out_between_the_logits_rows(cuda_device):
+    store = torch.zeros(7, 40, device="cuda")
+    x, s, _, _ = make(7, 16, "f32", seed=3, masks=False)
+    store[:, 3:19] = x
+    r = symbol_logprobs(store[:, 3:19], s)
+    want = symbol_logprobs_grad(x, s, r.lse, r.entropy, -1.0)
+    got = symbol_logprobs_grad(store[:, 3:19], s, r.lse, r.entropy, -1.0, out=store[:, 20:36])
+    assert torch.equal(got, want) and torch.equal(store[:, 3:19], x) and (store[:, 36:] == 0).all()
+    for out in (store[:, 4:20], store.view(-1)[1:1 + 7 * 32].view(7, 32)[:, :16]):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            symbol_logprobs_grad(store[:, 3:19], s, r.lse, r.entropy, -1.0, out=out)
+
+
+def test_first_call_inside_a_capture(cuda_device):
+    """A fresh process whose first use of the kernels is a captured one."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = (
+        "import torch\n"
+        "from neural_block_textures_b200 import AdamW, symbol_logprobs, symbol_logprobs_grad\n"
+        "x = torch.randn(50, 300, device='cuda'); s = torch.zeros(50, dtype=torch.int32, device='cuda')\n"
+        "dl = torch.full((50,), -1.0, device='cuda'); opt = AdamW([x], state_bits=8, weight_decay=0.0)\n"
+        "it = torch.zeros(1, dtype=torch.int64, device='cuda'); g = torch.cuda.CUDAGraph(); torch.cuda.synchronize()\n"
+        "with torch.cuda.graph(g):\n"
+        "    r = symbol_logprobs(x, s, topk=3); d = symbol_logprobs_grad(x, s, r.lse, r.entropy, dl); it.add_(1); opt.step(it, 0.1, [d])\n"
+        "before = x.clone(); g.replay(); torch.cuda.synchronize()\n"
+        "moved = before - x; ok = (moved.abs() - 0.1).abs() < 1e-3\n"
+        "assert ok[d.abs() > 1e-4].all() and torch.equal(moved[d.abs() > 1e-4].sign(), d[d.abs() > 1e-4].sign()); print('fine')\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parent.parent)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
+
+
+def test_rate_under_the_counts_is_the_progress_prints(cuda_device):
+    """Level 0's palette indices rated under the logarithms of their counts: the mean code length and the entropy are the
+    order-0 figure that print_stats gives for the level. Every cell shares one row of logits (row stride 0)."""
+    from neural_block_textures_b200 import Trainer
+
+    from .helpers import spec_named, target_for
+    for name in ("cfg2", "cfg3", "generic"):
+        spec = spec_named(name)
+        z, p = spec.init_params()
+        with Trainer() as tr:
+            ok, why = tr.init(spec.model_desc(), z, p, target_for(spec))
+            assert ok, why
+            for it in range(1, 4):
+                tr.mlp_step(it, 0.02, 0.005, 16, 256)
+                tr.qat_search()
+            stats, _ = tr.print_stats()
+            z, _ = tr.download_model()
+        level = spec.levels[0]
+        bits = entropy = 0.0
+        for c, depth in enumerate(spec.qat_bits):
+            values = z[:level.size].reshape(-1, level.C)[:, c]
+            index = torch.tensor(np.rint((values.astype(np.float64) + 1) / 2 * ((1 << depth) - 1)).astype(np.uint8), device="cuda")
+            count = torch.bincount(index.long(), minlength=1 << depth)
+            r = symbol_logprobs(count.float().log()[None].expand(len(index), -1), index)
+            bits += -r.logp.double().sum().item() / math.log(2)
+            entropy += r.entropy[0].double().item() * len(index) / math.log(2)
+        # log of a count, log of their sum and their difference: a few 2^-24 of log(4096) each
+        for got in (bits, entropy):
+            assert abs(got / (spec.W * spec.H) - stats.bpp_ctx_level0) < 2e-5 * max(stats.bpp_ctx_level0, 1.0), name
+
+
 def test_rows_behind_32_bits(cuda_device):
     """Offsets past 2^32 elements: the last rows of 4.3 G logits."""
     v = 65536

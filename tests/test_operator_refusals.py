@@ -60,6 +60,12 @@ def test_bad_arguments():
     assert "stride" in gradient(desc(), dlogp_stride=-1)[1]
     assert gradient(desc(), dentropy=BUF) == (0, "null buffer")
     assert "aligned" in gradient(desc(dtype=1), dx=BUF + 1)[1]
+    # dlogits over the logits (BUF): shifted, of another stride, or over a broadcast row
+    for kw in (dict(dx=BUF + 4), dict(dx=BUF + 4 * 8), dict(dx=BUF, dx_stride=9), dict(dx=BUF - 4)):
+        assert "overlaps" in gradient(desc(), **kw)[1]
+    assert "overlaps" in gradient(desc(row_stride=0), dx=BUF)[1]
+    assert "overlaps" in gradient(desc(row_stride=20), dx=BUF + 4 * 13, dx_stride=20)[1]
+    assert "overlaps" not in gradient(desc(rows=0))[1]
     # nothing to do is no refusal, and touches no device
     assert forward(desc(rows=0), logits=None)[0] == 1 and gradient(desc(rows=0))[0] == 1
 
