@@ -151,6 +151,7 @@ __device__ __forceinline__ void resolve(Scalars& c) {
 // elementary operations; the parameter's update uses the hardware's approximate square root and reciprocal (a few units
 // in the last place of an update that is itself a small part of the parameter).
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+template <bool FLUSH>
 __device__ __forceinline__ void update2(const Scalars& c, float2& p, float2 g, float2& m, float2& v) {
     // a b + c as (a b) * one + c, one = 1 only at run time: a packed product and a packed sum would be joined to one rounding
     const float2 one = both(c.one);
@@ -158,20 +159,32 @@ __device__ __forceinline__ void update2(const Scalars& c, float2& p, float2 g, f
     m = __ffma2_rn(__fmul2_rn(m, both(c.b1)), one, __fmul2_rn(g, both(c.omb1)));
     v = __ffma2_rn(__fmul2_rn(v, both(c.b2)), one, __fmul2_rn(__fmul2_rn(g, g), both(c.omb2)));
     float2 r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
+    if constexpr (FLUSH) {
+        asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
+        asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
+    } else {
+        asm("sqrt.approx.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
+        asm("sqrt.approx.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
+    }
     r = __ffma2_rn(r, both(c.inv), both(c.eps));   // between 2^-75 (or 0) and 2^65: its reciprocal needs no care for subnormals
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r.x));
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r.y));
     p = __ffma2_rn(__fmul2_rn(m, both(-c.step)), r, __fmul2_rn(p, both(c.decay)));
 }
+template <bool FLUSH>
 __device__ __forceinline__ void update(const Scalars& c, float (&p)[kVec], const float (&g)[kVec], float (&m)[kVec], float (&v)[kVec]) {
 #pragma unroll
     for (int i = 0; i < kVec; i += 2) {   // two elements to an instruction
         float2 p2 = make_float2(p[i], p[i + 1]), m2 = make_float2(m[i], m[i + 1]), v2 = make_float2(v[i], v[i + 1]);
-        update2(c, p2, make_float2(g[i], g[i + 1]), m2, v2);
+        update2<FLUSH>(c, p2, make_float2(g[i], g[i + 1]), m2, v2);
         p[i] = p2.x; p[i + 1] = p2.y; m[i] = m2.x; m[i + 1] = m2.y; v[i] = v2.x; v[i + 1] = v2.y;
     }
+}
+// A subnormal v has a root below 2^-63, and with inv <= 2^7 (beta2 up to 0.9999 at the first step) adds less than 2^-56 to
+// the denominator: nothing beside eps from 2^-33 on, so its root may be flushed to zero there (three instructions less).
+__device__ __forceinline__ void update(const Scalars& c, float (&p)[kVec], const float (&g)[kVec], float (&m)[kVec], float (&v)[kVec]) {
+    if (c.eps >= 1.1641532e-10f && c.inv <= 128.0f) update<true>(c, p, g, m, v);
+    else update<false>(c, p, g, m, v);
 }
 
 // ---- 8-bit codes
@@ -213,8 +226,8 @@ struct State8 {
 
 // Where the 16 random bits of each value come from: the low half of word i is m's, the high half v's.
 struct Noise {          // two neighbouring elements share a 64-bit draw; i counts the lane's elements
-    uint64_t key, pair; // pair: half the index of the lane's first element (which is even)
-    __device__ __forceinline__ uint64_t operator()(int i) const { return draw64(key, pair + (uint64_t)(i / 4 * 64 + i % 4 / 2)); }
+    uint64_t first;     // key + (index of the lane's first pair) * golden: draw64(key, pair + k) = mix64(first + k golden)
+    __device__ __forceinline__ uint64_t operator()(int i) const { return mix64(first + (uint64_t)(i / 4 * 64 + i % 4 / 2) * kGolden64); }
 };
 struct Nearest {        // half a grid step
     __device__ __forceinline__ uint64_t operator()(int) const { return 0x8000800080008000ull; }
@@ -248,7 +261,7 @@ __device__ __noinline__ void encode_slow(const float* m, const float* v, R rnd, 
 // code in its top byte. A value that is not finite, or that may round to infinity, shows in the largest t.
 template <class R>
 __device__ __forceinline__ void encode(const State8& s, long long at, int lane, const float (&m)[kVec], const float (&v)[kVec], const R& rnd) {
-    uint32_t tm[kVec], tv[kVec], most_m = 0, most_v = 0;
+    uint32_t tm[kVec], tv[kVec], most_m = 0, most_v = 0, least_v = 1;
 #pragma unroll
     for (int i = 0; i < kVec; i += 2) {
         const uint64_t r = rnd(i);
@@ -256,9 +269,11 @@ __device__ __forceinline__ void encode(const State8& s, long long at, int lane, 
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             tm[i + k] = (__float_as_uint(m[i + k]) & 0x7fffffffu) + __byte_perm(w[k], 0, 0x4410) * 16u;
-            tv[i + k] = (__float_as_uint(v[i + k]) & 0x7fffffffu) + __byte_perm(w[k], 0, 0x4432) * 16u;
-            most_m = max(most_m, tm[i + k]); most_v = max(most_v, tv[i + k]);
+            tv[i + k] = __float_as_uint(v[i + k]) + __byte_perm(w[k], 0, 0x4432) * 16u;   // v has no sign, but a NaN's
         }
+        most_m = __vimax3_u32(most_m, tm[i], tm[i + 1]);
+        most_v = __vimax3_u32(most_v, tv[i], tv[i + 1]);
+        least_v = __vimin3_u32(least_v, __float_as_uint(v[i]), __float_as_uint(v[i + 1]));
     }
     most_m = __reduce_max_sync(kFull, most_m);
     most_v = __reduce_max_sync(kFull, most_v);
@@ -268,10 +283,13 @@ __device__ __forceinline__ void encode(const State8& s, long long at, int lane, 
         bv = most_v >> 20; bv = bv > kTopV ? bv - kTopV : 0u;
         const uint32_t bm20 = bm << 20, bv20 = bv << 20;
 #pragma unroll
-        for (int i = 0; i < kVec; i++) {
-            tm[i] = (max(tm[i], bm20) * 16u - bm20 * 16u) | (__float_as_uint(m[i]) & 0x80000000u);
-            const uint32_t least = min(__float_as_uint(v[i]), 1u) * (1u << 20) + bv20;   // code 1 for v > 0
-            tv[i] = max(tv[i], least) * 16u - bv20 * 16u;
+        for (int i = 0; i < kVec; i++) tm[i] = (max(tm[i], bm20) * 16u - bm20 * 16u) | (__float_as_uint(m[i]) & 0x80000000u);
+        if (least_v) {   // v > 0 has at least code 1
+#pragma unroll
+            for (int i = 0; i < kVec; i++) tv[i] = max(tv[i], bv20 + (1u << 20)) * 16u - bv20 * 16u;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVec; i++) tv[i] = max(tv[i], min(__float_as_uint(v[i]), 1u) * (1u << 20) + bv20) * 16u - bv20 * 16u;
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -359,13 +377,13 @@ __device__ __forceinline__ void step_block(const StepArgs<N>& a, const Scalars& 
             for (int i = 0; i < kVec; i++)
                 if (i / 4 * 128 + i % 4 >= left) m[i] = v[i] = 0.0f;   // behind the tensor's end
         }
-        encode(s, st, lane, m, v, Noise{stream_key(c.seed, kStreamAdamW, c.it, (uint32_t)ch.tensor), (uint64_t)at >> 1});
+        encode(s, st, lane, m, v, Noise{stream_key(c.seed, kStreamAdamW, c.it, (uint32_t)ch.tensor) + ((uint64_t)at >> 1) * kGolden64});
     }
 }
 
 // Parameters and gradients of one type are the usual case and take the compiled conversions; mixed ones choose per load.
 template <int BITS, int N>
-__global__ void __launch_bounds__(256, 4) k_adamw(const __grid_constant__ StepArgs<N> a) {
+__global__ void __launch_bounds__(256, BITS == 8 ? 5 : 4) k_adamw(const __grid_constant__ StepArgs<N> a) {
     const Chunk ch = a.chunks[blockIdx.x];
     const void* g = a.g[ch.tensor - a.first];
     void* p = a.p[ch.tensor - a.first];
