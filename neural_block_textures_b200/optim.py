@@ -14,6 +14,7 @@ int64 tensor and advance it there.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from array import array
 
 import torch
@@ -23,6 +24,7 @@ from .symbols import DTYPES, _call, _raw_stream
 
 _T = torch.Tensor
 _dtype_of = _T.dtype.__get__
+_pack_args = struct.Struct("6dqQ3Q").pack   # ntcb_adamw_args
 
 
 class AdamW:
@@ -69,6 +71,8 @@ class AdamW:
             raise RuntimeError("AdamW: " + why.value.decode())
         self.offsets = [int(self.lib.ntcb_adamw_offset(self.h, i)) for i in range(n + 1)]   # elements; the last is the total
         self.state = torch.zeros(self.lib.ntcb_adamw_state_bytes(self.h), dtype=torch.uint8, device=self.device)
+        if state_bits == 32:
+            self._mv = self.state.view(torch.float32).split(self.offsets[-1]) if self.offsets[-1] else (self.state.view(torch.float32),) * 2
 
     def close(self) -> None:
         if getattr(self, "h", None):
@@ -85,13 +89,11 @@ class AdamW:
         if not self.h:
             raise RuntimeError("AdamW: closed")
 
-    def _scalar(self, x, dtype: torch.dtype, name: str):
-        """(host value, device pointer) of a number or of a one-element device tensor."""
-        if not isinstance(x, torch.Tensor):
-            return x, None
+    def _scalar(self, x: torch.Tensor, dtype: torch.dtype, name: str) -> tuple[int, int]:
+        """(the host value's place holder, the device address) of a one-element device tensor."""
         if x.dtype != dtype or x.numel() != 1 or x.device != self.device:
             raise ValueError(f"AdamW.step: {name} as a tensor must be one {dtype} on {self.device}")
-        return None, x.data_ptr()
+        return 1, x.data_ptr()
 
     def _addresses(self, params, grads, live) -> tuple[array, array]:
         """The tensors' addresses, after checking them against the plan (`live`: which of its tensors; None: all)."""
@@ -120,22 +122,20 @@ class AdamW:
             pp, gg = array("Q", bytes(8 * len(params))), array("Q", bytes(8 * len(params)))
             for i, p, g in zip(live, *self._addresses([params[i] for i in live], [grads[i] for i in live], live)):
                 pp[i], gg[i] = p, g
-        it, it_dev = self._scalar(it, torch.int64, "it")
-        lr, lr_dev = self._scalar(lr, torch.float32, "lr")
-        scale, scale_dev = self._scalar(grad_scale, torch.float32, "grad_scale")
-        args = abi.AdamWArgs(0.0 if lr is None else lr, self.betas[0], self.betas[1], self.eps, self.weight_decay,
-                             1.0 if scale is None else scale, 0 if it is None else it, self.seed & (1 << 64) - 1, it_dev, lr_dev, scale_dev)
-        _call(self.lib.ntcb_adamw_step, "AdamW.step", self.h, pp.buffer_info()[0], gg.buffer_info()[0], self.state.data_ptr(),
-              C.byref(args), _raw_stream(index))
+        it, it_dev = self._scalar(it, torch.int64, "it") if isinstance(it, _T) else (it, 0)
+        lr, lr_dev = self._scalar(lr, torch.float32, "lr") if isinstance(lr, _T) else (lr, 0)
+        grad_scale, scale_dev = self._scalar(grad_scale, torch.float32, "grad_scale") if isinstance(grad_scale, _T) else (grad_scale, 0)
+        args = _pack_args(lr, *self.betas, self.eps, self.weight_decay, grad_scale, it, self.seed & 0xFFFFFFFFFFFFFFFF, it_dev, lr_dev, scale_dev)
+        _call(self.lib.ntcb_adamw_step, "AdamW.step", self.h, pp.buffer_info()[0], gg.buffer_info()[0], self.state.data_ptr(), args,
+              _raw_stream(index))
 
     def moments_flat(self) -> tuple[torch.Tensor, torch.Tensor]:
         """(m, v) as flat float32 tensors, tensor i at offsets[i]: the state itself with 32 bits, the values that the
         codes stand for with 8."""
         self._open()
-        total = self.offsets[-1]
         if self.state_bits == 32:
-            mv = self.state.view(torch.float32)
-            return mv[:total], mv[total:]
+            return self._mv
+        total = self.offsets[-1]
         m = torch.empty(total, dtype=torch.float32, device=self.device)
         v = torch.empty_like(m)
         _call(self.lib.ntcb_adamw_get_moments, "AdamW.moments", self.h, self.state.data_ptr(), m.data_ptr(), v.data_ptr(),
