@@ -232,24 +232,21 @@ __device__ __forceinline__ void write_row(const RowArgs& a, long long r, const T
 // ------------------------------------------------------------------------------------------------------------- keys
 
 // A logit and its position as one integer: larger value first, then the lower position; 0 is no logit. The value part
-// orders as the numbers do (-0 and +0 are one): sign and magnitude turned into an offset number. 16-bit logits at up to
-// 2^16 positions fit 32 bits (one compare, one shuffle, one warp reduction), others take 64.
-template <class T, class K>
-__device__ __forceinline__ K key_of_bits(uint32_t b, uint32_t pos) {   // b: the logit's bits, at the top of the word
-    const uint32_t s = (uint32_t)((int32_t)b >> 31);
-    if constexpr (sizeof(K) == 4) return (((b & 0x7fff0000u) ^ s) - s) + (0x8000ffffu - pos);
-    else return ((K)((((b & 0x7fffffffu) ^ s) - s) + 0x80000000u) << 32) | (uint32_t)~pos;
-}
+// orders as the numbers do: all bits of a negative one turned, the sign of a positive one (-0 is made +0 first). 16-bit
+// logits at up to 2^16 positions fit 32 bits (one compare, one shuffle, one warp reduction), others take 64.
 template <class T, class K>
 __device__ __forceinline__ K key_of(float x, int pos) {
-    if constexpr (std::is_same_v<T, __half> && sizeof(K) == 4) return key_of_bits<T, K>((uint32_t)__half_as_ushort(__float2half_rn(x)) << 16, (uint32_t)pos);
-    else return key_of_bits<T, K>(__float_as_uint(x), (uint32_t)pos);
+    uint32_t b = __float_as_uint(x + 0.0f);
+    if constexpr (std::is_same_v<T, __half> && sizeof(K) == 4) b = (uint32_t)__half_as_ushort(__float2half_rn(x + 0.0f)) << 16;
+    const uint32_t o = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+    if constexpr (sizeof(K) == 4) return (o & 0xffff0000u) | (0xffffu - (uint32_t)pos);
+    else return ((K)o << 32) | (uint32_t)~pos;
 }
 template <class T, class K>
 __device__ __forceinline__ float key_value(K k) {
-    uint32_t o = sizeof(K) == 4 ? (uint32_t)k & 0xffff0000u : (uint32_t)((unsigned long long)k >> 32);
-    o -= 0x80000000u;
-    const uint32_t s = (uint32_t)((int32_t)o >> 31), b = ((o ^ s) - s) | (s & 0x80000000u);
+    const uint32_t o = sizeof(K) == 4 ? (uint32_t)k & 0xffff0000u : (uint32_t)((unsigned long long)k >> 32);
+    uint32_t b = o ^ ((uint32_t)((int32_t)~o >> 31) | 0x80000000u);
+    if constexpr (sizeof(K) == 4) b &= 0xffff0000u;
     if constexpr (std::is_same_v<T, __half> && sizeof(K) == 4) return __half2float(__ushort_as_half((unsigned short)(b >> 16)));
     else return __uint_as_float(b);
 }
@@ -258,14 +255,25 @@ __device__ __forceinline__ int key_index(K k) {
     if constexpr (sizeof(K) == 4) return (int)(0xffffu - (k & 0xffffu));
     else return (int)(~(uint32_t)k);
 }
-// The N keys of a vector whose first element has position pos.
+// The keys of a vector whose first element has position pos (known when compiled). Pairs of 16-bit logits are turned
+// together, and products and sums take what they can off the logic unit, which bounds the kernels that sort.
 template <class T, class K>
 __device__ __forceinline__ void keys_of(const uint4& a, int pos, K* k) {
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        if constexpr (sizeof(T) == 4) k[i] = key_of_bits<T, K>(w[i], (uint32_t)(pos + i));
-        else { k[2 * i] = key_of_bits<T, K>(w[i] << 16, (uint32_t)(pos + 2 * i)); k[2 * i + 1] = key_of_bits<T, K>(w[i] & 0xffff0000u, (uint32_t)(pos + 2 * i + 1)); }
+        if constexpr (sizeof(T) == 4) k[i] = key_of<T, K>(__uint_as_float(w[i]), pos + i);
+        else {
+            typedef typename std::conditional<std::is_same_v<T, __half>, __half2, __nv_bfloat162>::type P;
+            P p;
+            uint32_t b;
+            memcpy(&p, &w[i], 4);
+            if constexpr (std::is_same_v<T, __half>) p = __hadd2(p, __float2half2_rn(0.0f)); else p = __hadd2(p, __float2bfloat162_rn(0.0f));
+            memcpy(&b, &p, 4);
+            const uint32_t o = b ^ (((b >> 15) & 0x00010001u) * 0x7fffu + 0x80008000u);
+            k[2 * i] = o * 65536u + (0xffffu - (uint32_t)(pos + 2 * i));
+            k[2 * i + 1] = (o & 0xffff0000u) | (0xffffu - (uint32_t)(pos + 2 * i + 1));
+        }
     }
 }
 template <class T, class K>
@@ -474,8 +482,10 @@ __device__ __forceinline__ void rate_row(const RowArgs& a, const RowIn<T, E / VE
     } else if constexpr (L > 1) {
         K k[E];
 #pragma unroll
-        for (int c = 0; c < C; c++) keys_of<T>(raw[c], (c * G + lane) * N, k + c * N);
+        for (int c = 0; c < C; c++) keys_of<T>(raw[c], c * G * N, k + c * N);
         largest_keys<E, L>(k);
+#pragma unroll
+        for (int i = 0; i < L; i++) k[i] -= (K)(lane * N);   // the lane's part of the positions
         if constexpr (G == 1) {
 #pragma unroll
             for (int j = 0; j < L; j++)
@@ -879,11 +889,12 @@ cudaError_t launch_long(const RowArgs& a, int C, cudaStream_t s) {
 template <class T, class K>
 cudaError_t launch_long(const RowArgs& a, int span, cudaStream_t s, int sms) {
     // Warps to a row: eight, fewer as far as rows fill the GPU (24 warps an SM) or threads would not get two vectors. At
-    // 2048 x 65536 bf16 two took 55 us, eight 57; at 16384 x 4096 one took 30 us, eight 90.
+    // 2048 x 65536 bf16 two took 54 us, eight 57; at 16384 x 4096 one took 30 us, eight 90. With many alternatives a
+    // little more threads (32 warps an SM): their maxima bound the row better (20 of them: two warps 74 us, four 63).
     // CTAs to a row: where rows are few, parts of 8192 logits or more on up to eight CTAs. 16 x 65536 took 5.2 us with eight,
     // but 148 x 8192 8.6 us with four against 4.0 with one: clusters start slowly.
     int W = 8, C = 1;
-    while (W > 1 && (span < 64 * W * VEC<T> || a.rows * W / 2 >= 24ll * sms)) W /= 2;
+    while (W > 1 && (span < 64 * W * VEC<T> || a.rows * W / 2 >= (a.topk > 8 ? 32ll : 24ll) * sms)) W /= 2;
     if (W == 8)
         while (C < 8 && a.V / (C * 2) >= 8192 && a.rows * C * 2 <= 4 * sms) C *= 2;
     if (W == 1) return launch_long<T, K, 1, 4>(a, 1, s);
