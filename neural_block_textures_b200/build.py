@@ -1,12 +1,15 @@
 """Builds libntc_b200.so (the CUDA kernels, the host engine, the C ABI and the ntc_cuda::Trainer
-class) in-tree with nvcc for sm_100a. Run `python -m neural_block_textures_b200.build`."""
+class) in-tree with nvcc for sm_100a, and libntc_b200_torch.so (the host side of the operators on torch tensors) with
+the C++ compiler. Run `python -m neural_block_textures_b200.build`."""
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -15,6 +18,8 @@ CSRC = PKG / "csrc"
 OUT_DIR = PKG / "_lib"
 BUILD_DIR = PKG / "_build"
 LIB = OUT_DIR / "libntc_b200.so"
+TORCH_LIB = OUT_DIR / "libntc_b200_torch.so"
+TORCH_SOURCE = "torch_host.cpp"
 SOURCES = ["kernels_mlp.cu", "kernels_tc.cu", "kernels_latent.cu", "kernels_snap.cu", "kernels_stats.cu", "engine.cu",
            "ntcb_format.cpp", "ntcb_decoder.cu",
            "static_scratch.cu", "nccl_link.cpp", "p2p_exchange.cu", "device_cache.cu", "symbol_logprob.cu",
@@ -57,16 +62,46 @@ def _compile(src: str, verbose: bool) -> Path:
     return obj
 
 
+def _compile_torch_host() -> Path:
+    """torch_host.cpp against the installed torch's headers."""
+    s = CSRC / TORCH_SOURCE
+    obj = BUILD_DIR / (TORCH_SOURCE + ".o")
+    if not _stale(obj, _deps(s)):
+        return obj
+    torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    cuda = Path(nvcc()).resolve().parent.parent
+    inc = [torch / "include", torch / "include" / "torch" / "csrc" / "api" / "include", cuda / "include", sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", *[f"-I{d}" for d in inc], "-c", str(s), "-o", str(obj)]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for {TORCH_SOURCE}:\n{r.stdout}\n{r.stderr}")
+    return obj
+
+
+def _link_torch_host(obj: Path) -> None:
+    if not _stale(TORCH_LIB, [obj, LIB]):
+        return
+    torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", str(TORCH_LIB), str(obj), f"-L{OUT_DIR}", "-l:" + LIB.name, "-Wl,-rpath,$ORIGIN",
+           f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+
+
 def build(verbose: bool = False) -> Path:
     OUT_DIR.mkdir(exist_ok=True)
     BUILD_DIR.mkdir(exist_ok=True)
-    with cf.ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with cf.ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
+        host = ex.submit(_compile_torch_host)
         objs = list(ex.map(lambda s: _compile(s, verbose), SOURCES))
+        host_obj = host.result()
     if _stale(LIB, objs):
         cmd = [nvcc(), *GENCODE, "-shared", "-Xcompiler", "-fPIC", "-o", str(LIB), *map(str, objs), "-cudart", "static"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    _link_torch_host(host_obj)
     return LIB
 
 

@@ -1,0 +1,117 @@
+// The host side of the operators on torch tensors (symbols.py, optim.py) for calls that are all host work: a Python call per
+// tensor or argument costs 40 ns to 2 us, which is 15 us for one small rating and 130 us for an AdamW step over 300
+// tensors. These functions look at the same things and make the same calls of the C ABI (include/ntc_b200.h). Anything
+// but the plain case is left to the Python code, which names what is wrong: they return None (or an index) then.
+// Called through ctypes.PyDLL, so with the interpreter's lock held; a Python exception that is set is raised there.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cstdint>
+
+#include "../../include/ntc_b200.h"
+
+namespace {
+
+int dtype_code(at::ScalarType t) {
+    return t == at::kFloat ? NTCB_F32 : t == at::kHalf ? NTCB_F16 : t == at::kBFloat16 ? NTCB_BF16 : -1;
+}
+int symbol_code(at::ScalarType t) {
+    return t == at::kByte ? NTCB_SYM_U8 : t == at::kShort ? NTCB_SYM_I16 : t == at::kInt ? NTCB_SYM_I32 : t == at::kLong ? NTCB_SYM_I64 : -1;
+}
+bool plain(PyObject* o) { return THPVariable_Check(o) && THPVariable_Unpack(o).layout() == at::kStrided; }
+
+// The description of plain logits [n, V] and symbols [n] on one CUDA device; false for anything else.
+bool describe(PyObject* logits, PyObject* symbols, ntcb_symbol_desc& d) {
+    if (!plain(logits) || !plain(symbols)) return false;
+    const at::Tensor &x = THPVariable_Unpack(logits), &s = THPVariable_Unpack(symbols);
+    if (!x.is_cuda() || x.dim() != 2 || s.dim() != 1 || s.device() != x.device() || s.size(0) != x.size(0)) return false;
+    const int64_t n = x.size(0), v = x.size(1);
+    d = ntcb_symbol_desc{x.get_device(), dtype_code(x.scalar_type()), symbol_code(s.scalar_type()), 0, n, v, n > 1 ? x.stride(0) : v, s.stride(0)};
+    return d.dtype >= 0 && d.symbol_type >= 0 && v >= 1 && (v == 1 || x.stride(1) == 1);
+}
+// A float tensor [n] on the logits' device.
+bool per_row(PyObject* o, const ntcb_symbol_desc& d) {
+    if (!plain(o)) return false;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    return t.is_cuda() && t.get_device() == d.device && t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == d.rows;
+}
+void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream(); }
+
+PyObject* failed(const char* name, const char* why) {
+    PyErr_Format(PyExc_RuntimeError, "%s: %s", name, why);
+    return nullptr;
+}
+
+}  // namespace
+
+extern "C" {
+
+// (logp, entropy, lse, top_ids, top_logp), or None.
+PyObject* ntcb_host_logprobs(PyObject* logits, PyObject* symbols, int topk) {
+    ntcb_symbol_desc d;
+    if (!describe(logits, symbols, d) || topk < 0 || topk > NTCB_MAX_TOPK || topk > d.vocab) Py_RETURN_NONE;
+    try {
+        const at::Tensor &x = THPVariable_Unpack(logits), &s = THPVariable_Unpack(symbols);
+        const auto f = at::TensorOptions().dtype(at::kFloat).device(x.device());
+        const at::Tensor out[5] = {at::empty({d.rows}, f), at::empty({d.rows}, f), at::empty({d.rows}, f),
+                                   at::empty({d.rows, topk}, f.dtype(at::kInt)), at::empty({d.rows, topk}, f)};
+        char why[256];
+        if (!ntcb_symbol_logprobs(&d, x.data_ptr(), s.data_ptr(), topk, out[0].data_ptr<float>(), out[1].data_ptr<float>(),
+                                  out[2].data_ptr<float>(), out[3].data_ptr<int>(), out[4].data_ptr<float>(), stream_of(d.device), why, sizeof(why)))
+            return failed("symbol_logprobs", why);
+        PyObject* r = PyTuple_New(5);
+        if (!r) return nullptr;
+        for (int i = 0; i < 5; i++) {
+            PyObject* t = THPVariable_Wrap(out[i]);
+            if (!t) { Py_DECREF(r); return nullptr; }
+            PyTuple_SET_ITEM(r, i, t);
+        }
+        return r;
+    } catch (const std::exception& e) { return failed("symbol_logprobs", e.what()); }
+}
+
+// The gradient in a new tensor, or None. entropy and dentropy may be None.
+PyObject* ntcb_host_logprobs_grad(PyObject* logits, PyObject* symbols, PyObject* lse, PyObject* entropy, PyObject* dlogp, PyObject* dentropy) {
+    ntcb_symbol_desc d;
+    if (!describe(logits, symbols, d) || !per_row(lse, d) || !per_row(dlogp, d)) Py_RETURN_NONE;
+    const bool with = dentropy != Py_None;
+    if (with && (!per_row(dentropy, d) || !per_row(entropy, d) || !THPVariable_Unpack(entropy).is_contiguous())) Py_RETURN_NONE;
+    if (!THPVariable_Unpack(lse).is_contiguous()) Py_RETURN_NONE;
+    try {
+        const at::Tensor &x = THPVariable_Unpack(logits), &l = THPVariable_Unpack(dlogp);
+        const at::Tensor out = at::empty({d.rows, d.vocab}, at::TensorOptions().dtype(x.scalar_type()).device(x.device()));
+        char why[256];
+        if (!ntcb_symbol_logprobs_grad(&d, x.data_ptr(), THPVariable_Unpack(symbols).data_ptr(), THPVariable_Unpack(lse).data_ptr<float>(),
+                                       with ? THPVariable_Unpack(entropy).data_ptr<float>() : nullptr, l.data_ptr<float>(), l.stride(0),
+                                       with ? THPVariable_Unpack(dentropy).data_ptr<float>() : nullptr,
+                                       with ? THPVariable_Unpack(dentropy).stride(0) : 0, out.data_ptr(), d.vocab, stream_of(d.device), why, sizeof(why)))
+            return failed("symbol_logprobs_grad", why);
+        return THPVariable_Wrap(out);
+    } catch (const std::exception& e) { return failed("symbol_logprobs_grad", e.what()); }
+}
+
+// The addresses of n parameters and gradients (lists; a gradient may be None: 0 for both) after checking sizes, types,
+// layout and device. Returns -1, or the index of the first tensor that does not fit, or -2 when the lists do not.
+int ntcb_host_addresses(PyObject* params, PyObject* grads, int n, const long long* sizes, const int* param_types, const int* grad_types,
+                        int device, uint64_t* pp, uint64_t* gg) {
+    if (!PyList_Check(params) || !PyList_Check(grads) || PyList_GET_SIZE(params) != n || PyList_GET_SIZE(grads) != n) return -2;
+    const auto fits = [&](PyObject* o, long long size, int type) {
+        if (!plain(o)) return false;
+        const at::Tensor& t = THPVariable_Unpack(o);
+        return t.numel() == size && dtype_code(t.scalar_type()) == type && t.is_contiguous() && t.is_cuda() && t.get_device() == device;
+    };
+    try {
+        for (int i = 0; i < n; i++) {
+            PyObject *p = PyList_GET_ITEM(params, i), *g = PyList_GET_ITEM(grads, i);
+            pp[i] = gg[i] = 0;
+            if (g == Py_None) continue;
+            if (!fits(p, sizes[i], param_types[i]) || !fits(g, sizes[i], grad_types[i])) return i;
+            pp[i] = reinterpret_cast<uint64_t>(THPVariable_Unpack(p).data_ptr());
+            gg[i] = reinterpret_cast<uint64_t>(THPVariable_Unpack(g).data_ptr());
+        }
+    } catch (const std::exception&) { return -2; }
+    return -1;
+}
+
+}  // extern "C"

@@ -20,10 +20,9 @@ from array import array
 import torch
 
 from . import abi
-from .symbols import DTYPES, _call, _raw_stream
+from .symbols import DTYPES, _call, _host, _raw_stream
 
 _T = torch.Tensor
-_dtype_of = _T.dtype.__get__
 _pack_args = struct.Struct("6dqQ3Q").pack   # ntcb_adamw_args
 
 
@@ -64,9 +63,10 @@ class AdamW:
         self._grad_dtypes = [grad_dtype or p.dtype for p in self.params]
         self.lib = abi.load_library()
         why = C.create_string_buffer(256)
-        self.h = self.lib.ntcb_adamw_create(
-            self.device.index, n, (C.c_longlong * n)(*self._sizes), (C.c_int * n)(*[DTYPES[p.dtype] for p in self.params]),
-            (C.c_int * n)(*[DTYPES[t] for t in self._grad_dtypes]), state_bits, why, 256)
+        self._keep = ((C.c_longlong * n)(*self._sizes), (C.c_int * n)(*[DTYPES[p.dtype] for p in self.params]),
+                      (C.c_int * n)(*[DTYPES[t] for t in self._grad_dtypes]))
+        self._plan = tuple(C.addressof(a) for a in self._keep)
+        self.h = self.lib.ntcb_adamw_create(self._index, n, *self._keep, state_bits, why, 256)
         if not self.h:
             raise RuntimeError("AdamW: " + why.value.decode())
         self.offsets = [int(self.lib.ntcb_adamw_offset(self.h, i)) for i in range(n + 1)]   # elements; the last is the total
@@ -95,39 +95,26 @@ class AdamW:
             raise ValueError(f"AdamW.step: {name} as a tensor must be one {dtype} on {self.device}")
         return 1, x.data_ptr()
 
-    def _addresses(self, params, grads, live) -> tuple[array, array]:
-        """The tensors' addresses, after checking them against the plan (`live`: which of its tensors; None: all)."""
-        sizes, dtypes = (self._sizes, self._grad_dtypes) if live is None else ([self._sizes[i] for i in live], [self._grad_dtypes[i] for i in live])
-        if list(map(_T.numel, params)) != sizes or not all(map(_T.is_contiguous, params)):
-            raise ValueError("AdamW.step: a parameter's size or layout has changed")
-        if (list(map(_T.numel, grads)) != sizes or list(map(_dtype_of, grads)) != dtypes or not all(map(_T.is_contiguous, grads))
-                or not set(map(_T.get_device, grads)) <= {self._index}):
-            raise ValueError("AdamW.step: a gradient must be contiguous, on the parameters' device and of its parameter's size and the plan's type")
-        return array("Q", map(_T.data_ptr, params)), array("Q", map(_T.data_ptr, grads))
-
     def step(self, it, lr, grads=None, grad_scale=1.0) -> None:
         """Step number `it` (from 1) at learning rate `lr` with the gradients `grads` (default: each p.grad) times
         grad_scale; a None gradient leaves its tensor and moments alone. it, lr and grad_scale may be device tensors
         (int64, float32, float32)."""
         self._open()
-        if grads is None:
-            grads = [p.grad for p in self.params]
-        if len(grads) != len(self.params):
-            raise ValueError(f"AdamW.step: {len(self.params)} gradients are needed, not {len(grads)}")
-        params, index = self.params, self._index
-        try:
-            pp, gg = self._addresses(params, grads, None)
-        except TypeError:   # something in grads is no tensor: None is allowed
-            live = [i for i, g in enumerate(grads) if g is not None]
-            pp, gg = array("Q", bytes(8 * len(params))), array("Q", bytes(8 * len(params)))
-            for i, p, g in zip(live, *self._addresses([params[i] for i in live], [grads[i] for i in live], live)):
-                pp[i], gg[i] = p, g
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
+        n = len(self.params)
+        pp, gg = array("Q", bytes(8 * n)), array("Q", bytes(8 * n))
+        bad = _host.ntcb_host_addresses(self.params, grads, n, *self._plan, self._index, pp.buffer_info()[0], gg.buffer_info()[0])
+        if bad == -2:
+            raise ValueError(f"AdamW.step: {n} gradients are needed, not {len(grads)}")
+        if bad >= 0:
+            raise ValueError(f"AdamW.step: gradient {bad} must be a contiguous {self._grad_dtypes[bad]} tensor of {self._sizes[bad]} elements on "
+                             f"{self.device}, and its parameter as it was when the plan was made")
         it, it_dev = self._scalar(it, torch.int64, "it") if isinstance(it, _T) else (it, 0)
         lr, lr_dev = self._scalar(lr, torch.float32, "lr") if isinstance(lr, _T) else (lr, 0)
         grad_scale, scale_dev = self._scalar(grad_scale, torch.float32, "grad_scale") if isinstance(grad_scale, _T) else (grad_scale, 0)
         args = _pack_args(lr, *self.betas, self.eps, self.weight_decay, grad_scale, it, self.seed & 0xFFFFFFFFFFFFFFFF, it_dev, lr_dev, scale_dev)
         _call(self.lib.ntcb_adamw_step, "AdamW.step", self.h, pp.buffer_info()[0], gg.buffer_info()[0], self.state.data_ptr(), args,
-              _raw_stream(index))
+              _raw_stream(self._index))
 
     def moments_flat(self) -> tuple[torch.Tensor, torch.Tensor]:
         """(m, v) as flat float32 tensors, tensor i at offsets[i]: the state itself with 32 bits, the values that the

@@ -65,6 +65,24 @@ def _call(fn, name: str, *args) -> None:
         raise RuntimeError(f"{name}: {why.value.decode()}")
 
 
+def _load_host() -> C.PyDLL:
+    """The compiled host side (csrc/torch_host.cpp)."""
+    abi.load_library()
+    path = abi.LIB_PATH.with_name("libntc_b200_torch.so")
+    if not path.exists():
+        raise RuntimeError(f"{path.name} not found at {path}: build it with `python -m neural_block_textures_b200.build`")
+    lib = C.PyDLL(str(path))
+    o = C.py_object
+    lib.ntcb_host_logprobs.restype, lib.ntcb_host_logprobs.argtypes = o, [o, o, C.c_int]
+    lib.ntcb_host_logprobs_grad.restype, lib.ntcb_host_logprobs_grad.argtypes = o, [o] * 6
+    lib.ntcb_host_addresses.restype = C.c_int
+    lib.ntcb_host_addresses.argtypes = [o, o, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]
+    return lib
+
+
+_host = _load_host()
+
+
 def _per_row(x: torch.Tensor, n: int, device: int, name: str) -> torch.Tensor:
     if x.dtype is not torch.float32 or x.shape != (n,) or x.get_device() != device:
         raise ValueError(f"symbol_logprobs_grad: {name} must be a float32 tensor of [{n}] on the logits' device")
@@ -74,16 +92,13 @@ def _per_row(x: torch.Tensor, n: int, device: int, name: str) -> torch.Tensor:
 def symbol_logprobs(logits: torch.Tensor, symbols: torch.Tensor, topk: int = 0) -> SymbolLogprobs:
     """Log probabilities of `symbols` [n] under `logits` [n, V] with the rows' entropy, log-sum-exp and `topk` (0 .. 32,
     at most V) likeliest symbols, in one pass over the logits. Rows may be strided; a row's logits are contiguous."""
-    d, n, v, device = _desc(logits, symbols, "symbol_logprobs")
+    r = _host.ntcb_host_logprobs(logits, symbols, topk)
+    if r is not None:
+        return SymbolLogprobs(*r)
+    _, n, v, _ = _desc(logits, symbols, "symbol_logprobs")   # says what is wrong
     if not 0 <= topk <= min(abi.MAX_TOPK, v):
         raise ValueError(f"symbol_logprobs: topk must be 0 .. {min(abi.MAX_TOPK, v)} here, not {topk}")
-    # one allocation: a small call is mostly host work (2 us an allocation)
-    out = torch.empty(n * (3 + 2 * topk), dtype=torch.float32, device=logits.device)
-    logp, entropy, lse, top, ids = out.split_with_sizes((n, n, n, n * topk, n * topk))
-    p = out.data_ptr()
-    _call(abi.load_library().ntcb_symbol_logprobs, "symbol_logprobs", d, logits.data_ptr(), symbols.data_ptr(), topk,
-          p, p + 4 * n, p + 8 * n, p + 4 * n * (3 + topk), p + 12 * n, _raw_stream(device))
-    return SymbolLogprobs(logp, entropy, lse, ids.view(torch.int32).view(n, topk), top.view(n, topk))
+    raise ValueError("symbol_logprobs: logits and symbols must be strided tensors")
 
 
 def symbol_logprobs_grad(logits: torch.Tensor, symbols: torch.Tensor, lse: torch.Tensor, entropy: torch.Tensor | None,
@@ -93,6 +108,10 @@ def symbol_logprobs_grad(logits: torch.Tensor, symbols: torch.Tensor, lse: torch
     and entropy. dlogp / dentropy: [n] float32 (any stride, so an expanded scalar too) or a number for every row.
     out: where to write it, of the logits' shape and type; the logits themselves are allowed, memory
     that overlaps them otherwise is refused."""
+    if out is None and isinstance(dlogp, torch.Tensor) and (dentropy is None or isinstance(dentropy, torch.Tensor)):
+        r = _host.ntcb_host_logprobs_grad(logits, symbols, lse, entropy, dlogp, dentropy)
+        if r is not None:
+            return r
     d, n, v, device = _desc(logits, symbols, "symbol_logprobs_grad")
     dev = logits.device
     if not isinstance(dlogp, torch.Tensor):
