@@ -214,7 +214,7 @@ __device__ __forceinline__ RowOut finish_row(const Sums& q) {
     o.m = q.m;
     o.log_s = logf(q.s);
     o.lse = o.empty ? kNegInf : q.m + o.log_s;
-    o.entropy = o.empty ? 0.0f : o.log_s - q.u / q.s;
+    o.entropy = o.empty ? 0.0f : o.log_s - __fdividef(q.u, q.s);
     return o;
 }
 // The row's scalars, by one thread; t is its symbol (fetched with the row), xt the symbol's logit, NaN where there is none.
@@ -276,12 +276,14 @@ __device__ __forceinline__ void keys_of(const uint4& a, int pos, K* k) {
         }
     }
 }
+__device__ __forceinline__ void write_top(const RowArgs& a, long long r, int i, float v, int index, const RowOut& o) {
+    const bool none = o.bad || v == kNegInf;
+    a.top_ids[r * a.topk + i] = none ? -1 : index;
+    a.top_logp[r * a.topk + i] = o.bad ? NAN : none ? kNegInf : (v - o.m) - o.log_s;
+}
 template <class T, class K>
 __device__ __forceinline__ void write_top(const RowArgs& a, long long r, int i, K k, int shift, const RowOut& o) {
-    const float v = k ? key_value<T, K>(k) : kNegInf;
-    const bool none = o.bad || v == kNegInf;
-    a.top_ids[r * a.topk + i] = none ? -1 : key_index(k) - shift;
-    a.top_logp[r * a.topk + i] = o.bad ? NAN : none ? kNegInf : (v - o.m) - o.log_s;
+    write_top(a, r, i, k ? key_value<T, K>(k) : kNegInf, key_index(k) - shift, o);
 }
 
 // The largest key of G neighbouring lanes, in all of them.
@@ -479,6 +481,26 @@ __device__ __forceinline__ void rate_row(const RowArgs& a, const RowIn<T, E / VE
             a.top_ids[r] = none ? -1 : at - shift;
             a.top_logp[r] = o.bad ? NAN : none ? kNegInf : -o.log_s;
         }
+    } else if constexpr (L > 1 && G == 1 && C == 1 && sizeof(T) == 4) {
+        // four fp32 logits: neighbours change places where the upper one is larger, which keeps equal ones in order (and
+        // needs no 64-bit keys)
+        float v[4];
+        int id[4];
+        expand<T>(raw[0], v);
+#pragma unroll
+        for (int i = 0; i < 4; i++) id[i] = i - shift;
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+            for (int i = n % 2; i + 1 < 4; i += 2) {
+                const bool swap = v[i + 1] > v[i];
+                const float x = swap ? v[i + 1] : v[i], y = swap ? v[i] : v[i + 1];
+                const int ix = swap ? id[i + 1] : id[i], iy = swap ? id[i] : id[i + 1];
+                v[i] = x; v[i + 1] = y; id[i] = ix; id[i + 1] = iy;
+            }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (live && j < a.topk) write_top(a, r, j, v[j], id[j], o);
     } else if constexpr (L > 1) {
         K k[E];
 #pragma unroll
