@@ -668,6 +668,7 @@ __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, i
             sync();
             const int nwork = min(sh.nwork, kWork), each = U << lg;
             for (int item = tid; item < nwork * each; item += kThreads) {
+                if (*const_cast<volatile int*>(&sh.ncand) > kCand) break;   // the additions to it are one after another
                 const int w = sh.work[item / each], k = item % each;
                 const int c = first + w % kThreads + ((w / kThreads) * each + k) * kThreads;
                 if (c >= end) continue;
@@ -910,13 +911,16 @@ cudaError_t launch_long(const RowArgs& a, int C, cudaStream_t s) {
 
 template <class T, class K>
 cudaError_t launch_long(const RowArgs& a, int span, cudaStream_t s, int sms) {
-    // Warps to a row: eight, fewer as far as rows fill the GPU (24 warps an SM) or threads would not get two vectors. At
-    // 2048 x 65536 bf16 two took 54 us, eight 57; at 16384 x 4096 one took 30 us, eight 90. With many alternatives a
-    // little more threads (32 warps an SM): their maxima bound the row better (20 of them: two warps 74 us, four 63).
+    // Warps to a row: one for 1536 vectors (a warp's joins are paid once, and rows that have ended make place for others),
+    // more where that would leave an SM fewer than 10, and no more than leave a thread two vectors. Measured, bf16, warps
+    // 1 / 2 / 4 / 8: 12000 x 4099 29 / 38 / 41 / 66 us, 6000 x 16384 44 / 40 / 41 / 48, 2048 x 65536 74 / 54 / 55 / 52, 300 x
+    // 16384 12 / 7.9 / 6.1 / 6.1. Over 16 alternatives want more maxima than one warp's lanes have (12000 x 4099 with 32:
+    // 111 / 68 / 73 / 115 us).
+    const int vectors = (span + VEC<T> - 1) / VEC<T>;
+    int W = a.topk > 16 ? 2 : 1, C = 1;
+    while (W < 8 && (vectors > 1536 * W || a.rows * W < 10ll * sms) && vectors >= 64 * W * 2) W *= 2;
     // CTAs to a row: where rows are few, parts of 8192 logits or more on up to eight CTAs. 16 x 65536 took 5.2 us with eight,
     // but 148 x 8192 8.6 us with four against 4.0 with one: clusters start slowly.
-    int W = 8, C = 1;
-    while (W > 1 && (span < 64 * W * VEC<T> || a.rows * W / 2 >= (a.topk > 8 ? 32ll : 24ll) * sms)) W /= 2;
     if (W == 8)
         while (C < 8 && a.V / (C * 2) >= 8192 && a.rows * C * 2 <= 4 * sms) C *= 2;
     if (W == 1) return launch_long<T, K, 1, 4>(a, 1, s);
