@@ -933,21 +933,25 @@ template <class T>
 cudaError_t launch_rows(const RowArgs& a, cudaStream_t s, int sms) {
     constexpr int N = VEC<T>;
     const int span = row_span<T>(a.x, a.stride, a.V);
+    // Rows in registers as far as that is the faster way: without alternatives or with one up to 1024 elements; 16-bit logits
+    // with up to eight also (1024 bf16: 42 us for 2^25 logits, either way), with more up to 512 (512 with nine: 71 us, as long
+    // rows 90); fp32 logits, whose keys take 64 bits, up to 256 (257 with nine: 304 us, as long rows 162).
     bool done = false;
     if (a.topk == 0) {
         if (span <= N) { launch_lanes<T, 1, N, 0>(a, s); done = true; }
         else if (span <= 16) { launch_lanes<T, 1, 16, 0>(a, s); done = true; }
         else if (span <= 64) { launch_lanes<T, 4, 16, 0>(a, s); done = true; }
-        else if (span > 64) done = launch_lanes<T, 32, 0>(a, span, s);
+        else done = launch_lanes<T, 32, 0>(a, span, s);
     } else if (a.topk == 1) {
         if (span <= N) { launch_lanes<T, 1, N, 1>(a, s); done = true; }
-        else done = launch_lanes<T, sizeof(T) == 2 ? 32 : 16, 1>(a, span, s);
+        else done = launch_lanes<T, 32, 1>(a, span, s);
     } else if (a.topk <= 8) {
         if (span <= N) { launch_lanes<T, 1, N, N>(a, s); done = true; }
         else if (span <= 8) { launch_lanes<T, 1, 8, 8>(a, s); done = true; }
         else if (span <= 16) { launch_lanes<T, 1, 16, 8>(a, s); done = true; }
-        else done = launch_lanes<T, sizeof(T) == 2 ? 32 : 16, 8>(a, span, s);
-    } else {
+        else if (sizeof(T) == 2) done = launch_lanes<T, sizeof(T) == 2 ? 32 : 16, 8>(a, span, s);
+        else if (span <= 256) done = launch_lanes<T, 16, 8>(a, span, s);
+    } else if (sizeof(T) == 2 || span <= 256) {
         done = launch_lanes<T, 16, 16>(a, span, s);
     }
     if (!done) {
