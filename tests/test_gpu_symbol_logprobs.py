@@ -109,6 +109,15 @@ def test_forward_lengths(v, dtype, cuda_device):
         check_forward(*make(19, v, dtype, seed=v, symbol=torch.int32), topk)
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("v", [4, 6, 15, 30, 90, 200, 256, 300, 700, 1200, 9000])
+def test_forward_numbers_of_alternatives(v, dtype, cuda_device):
+    x, s, x64, s64 = make(17, v, dtype, seed=v + 1)
+    for topk in (2, 3, 4, 8, 9, 16, 17, 31):
+        if topk <= v:
+            check_forward(x, s, x64, s64, topk)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("n, v", [(1, 65536), (1, 16385), (2, 30011), (3, 65535), (9, 20000), (40, 9001), (700, 2100), (1, 300007)])
 def test_forward_long_rows(n, v, dtype, cuda_device):
