@@ -933,10 +933,11 @@ cudaError_t launch_long(const RowArgs& a, int span, cudaStream_t s, int sms) {
     // Warps to a row: one for 1536 vectors (a warp's joins are paid once, and rows that have ended make place for others),
     // more where that would leave an SM fewer than 10, and no more than leave a thread two vectors. Measured, bf16, warps
     // 1 / 2 / 4 / 8: 12000 x 4099 29 / 38 / 41 / 66 us, 6000 x 16384 44 / 40 / 41 / 48, 2048 x 65536 74 / 54 / 55 / 52, 300 x
-    // 16384 12 / 7.9 / 6.1 / 6.1. Over 16 alternatives want more maxima than one warp's lanes have (12000 x 4099 with 32:
-    // 111 / 68 / 73 / 115 us).
+    // 16384 12 / 7.9 / 6.1 / 6.1. Almost as many
+    // alternatives as a warp has lanes want more maxima than one warp gives (12000 x 4099: 61 us with 30; with 32 one warp 113,
+    // two 68), but where a lane holds few logits anyway (2^25 in rows of 1024: 88 against 116).
     const int vectors = (span + VEC<T> - 1) / VEC<T>;
-    int W = a.topk > 16 ? 2 : 1, C = 1;
+    int W = a.topk > 30 && span > 1024 ? 2 : 1, C = 1;
     while (W < 8 && (vectors > 1536 * W || a.rows * W < 10ll * sms) && vectors >= 64 * W * 2) W *= 2;
     // CTAs to a row: where rows are few, parts of 8192 logits or more on up to eight CTAs. 16 x 65536 took 5.2 us with eight,
     // but 148 x 8192 8.6 us with four against 4.0 with one: clusters start slowly.
