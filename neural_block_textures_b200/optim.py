@@ -148,8 +148,8 @@ class AdamW:
               self.state.data_ptr(), _raw_stream(self._index))
 
     def state_dict(self) -> dict:
-        """The state (a copy) with what it was laid out for."""
-        return {"state_bits": self.state_bits, "sizes": list(self._sizes), "state": self.state.clone()}
+        """The state (a copy) with what it was laid out for, and the seed of its rounding."""
+        return {"state_bits": self.state_bits, "sizes": list(self._sizes), "seed": self.seed, "state": self.state.clone()}
 
     def load_state_dict(self, d: dict) -> None:
         if d["state_bits"] != self.state_bits or list(d["sizes"]) != self._sizes:
@@ -157,3 +157,4 @@ class AdamW:
         if d["state"].dtype != torch.uint8 or d["state"].numel() != self.state.numel():
             raise ValueError("AdamW.load_state_dict: the state has another size")
         self.state.copy_(d["state"])
+        self.seed = d["seed"]

@@ -92,9 +92,10 @@ def _per_row(x: torch.Tensor, n: int, device: int, name: str) -> torch.Tensor:
 def symbol_logprobs(logits: torch.Tensor, symbols: torch.Tensor, topk: int = 0) -> SymbolLogprobs:
     """Log probabilities of `symbols` [n] under `logits` [n, V] with the rows' entropy, log-sum-exp and `topk` (0 .. 32,
     at most V) likeliest symbols, in one pass over the logits. Rows may be strided; a row's logits are contiguous."""
-    r = _host.ntcb_host_logprobs(logits, symbols, topk)
-    if r is not None:
-        return SymbolLogprobs(*r)
+    if 0 <= topk <= abi.MAX_TOPK:
+        r = _host.ntcb_host_logprobs(logits, symbols, topk)
+        if r is not None:
+            return SymbolLogprobs(*r)
     _, n, v, _ = _desc(logits, symbols, "symbol_logprobs")   # says what is wrong
     if not 0 <= topk <= min(abi.MAX_TOPK, v):
         raise ValueError(f"symbol_logprobs: topk must be 0 .. {min(abi.MAX_TOPK, v)} here, not {topk}")
