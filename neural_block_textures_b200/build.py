@@ -23,7 +23,7 @@ TORCH_SOURCE = "torch_host.cpp"
 SOURCES = ["kernels_mlp.cu", "kernels_tc.cu", "kernels_latent.cu", "kernels_snap.cu", "kernels_stats.cu", "engine.cu",
            "ntcb_format.cpp", "ntcb_decoder.cu",
            "static_scratch.cu", "nccl_link.cpp", "p2p_exchange.cu", "device_cache.cu", "symbol_logprob.cu",
-           "adamw.cu"]
+           "symbol_logprob_f32.cu", "symbol_logprob_f16.cu", "symbol_logprob_bf16.cu", "adamw.cu"]
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # No fast-math: the noise (logf / cosf / sqrtf), the sigmoid (expf) and every division must be CUDA's
 # IEEE / accurate versions for parity with the reference backend.
