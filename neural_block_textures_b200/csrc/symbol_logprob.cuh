@@ -873,28 +873,21 @@ template <class T, int G, int E, int L>
 void launch_lanes(const RowArgs& a, cudaStream_t s) {
     k_logprobs_lanes<T, G, E, L><<<(unsigned)ceil_div(a.rows, 256 / G), 256, 0, s>>>(a);
 }
-// Rows of up to 32 E elements: the fewest lanes that hold them (a row's joins and its end are paid per lane).
-template <class T, int E, int L>
-bool launch_lanes(const RowArgs& a, int span, cudaStream_t s) {
-    if (span <= E) launch_lanes<T, 1, E, L>(a, s);
-    else if (span <= 2 * E) launch_lanes<T, 2, E, L>(a, s);
-    else if (span <= 4 * E) launch_lanes<T, 4, E, L>(a, s);
-    else if (span <= 8 * E) launch_lanes<T, 8, E, L>(a, s);
-    else if (span <= 16 * E) launch_lanes<T, 16, E, L>(a, s);
-    else if (span <= 32 * E) launch_lanes<T, 32, E, L>(a, s);
-    else return false;
-    return true;
+// Rows of up to GMAX * E elements on G lanes or the fewest above that hold them (a row's joins and its end are paid per
+// lane); false for longer ones.
+template <class T, int G, int GMAX, int E, int L>
+bool launch_fit(const RowArgs& a, int span, cudaStream_t s) {
+    if (span <= G * E) { launch_lanes<T, G, E, L>(a, s); return true; }
+    if constexpr (G < GMAX) return launch_fit<T, 2 * G, GMAX, E, L>(a, span, s);
+    return false;
 }
-// Rows with alternatives of up to 1024 16-bit or 256 fp32 elements: 64 (32) to a lane, half of that where it fits one or two
-// lanes. Lanes with more elements pay a row's joins and its end less often: 2^18 x 256 bf16 with eight took 72 us with 64
-// a lane, 81 with 32; 2^18 x 64 took 29 and 24.
+// Rows with up to eight alternatives: 64 16-bit (32 fp32) elements a lane, half of that for rows of one or two lanes. Lanes
+// with more elements pay a row's joins and its end less often: 2^18 x 256 bf16 with eight took 72 us with 64 a lane, 81 with
+// 32; 2^18 x 64 took 29 and 24.
 template <class T, int L>
 bool launch_sorted(const RowArgs& a, int span, cudaStream_t s) {
-    constexpr int E = sizeof(T) == 2 ? 64 : 32;
-    if (span <= E / 2) launch_lanes<T, 1, E / 2, L>(a, s);
-    else if (span <= E) launch_lanes<T, 2, E / 2, L>(a, s);
-    else return launch_lanes<T, E, L>(a, span, s);
-    return true;
+    if constexpr (sizeof(T) == 2) return span <= 64 ? launch_fit<T, 1, 2, 32, L>(a, span, s) : launch_fit<T, 2, 16, 64, L>(a, span, s);
+    else return span <= 32 ? launch_fit<T, 2, 2, 16, L>(a, span, s) : launch_fit<T, 2, 8, 32, L>(a, span, s);
 }
 template <class T, class K, int W, int R>
 cudaError_t launch_long(const RowArgs& a, int C, cudaStream_t s) {
@@ -914,10 +907,10 @@ template <class T, class K>
 cudaError_t launch_long(const RowArgs& a, int span, cudaStream_t s, int sms) {
     // Warps to a row: one for 1536 vectors (a warp's joins are paid once, and rows that have ended make place for others),
     // more where that would leave an SM fewer than 10, and no more than leave a thread two vectors. Measured, bf16, warps
-    // 1 / 2 / 4 / 8: 12000 x 4099 29 / 38 / 41 / 66 us, 6000 x 16384 44 / 40 / 41 / 48, 2048 x 65536 74 / 54 / 55 / 52, 300 x
-    // 16384 12 / 7.9 / 6.1 / 6.1. Almost as many
-    // alternatives as a warp has lanes want more maxima than one warp gives (12000 x 4099: 61 us with 30; with 32 one warp 113,
-    // two 68), but where a lane holds few logits anyway (2^25 in rows of 1024: 88 against 116).
+    // 1 / 2 / 4 / 8: 12000 x 4099 29 / 38 / 41 / 66 us, 6000 x 16384 44 / 40 / 41 / 48, 2048 x 65536 74 / 54 / 55 / 52,
+    // 300 x 16384 12 / 7.9 / 6.1 / 6.1. Almost as many alternatives as a warp has lanes want more maxima than one warp gives
+    // (12000 x 4099: 61 us with 30; with 32 one warp 113, two 68), except where a lane holds few logits anyway (2^25 in rows
+    // of 1024: 88 with one warp, 116 with two).
     const int vectors = (span + VEC<T> - 1) / VEC<T>;
     int W = a.topk > 30 && span > 1024 ? 2 : 1, C = 1;
     while (W < 8 && (vectors > 1536 * W || a.rows * W < 10ll * sms) && vectors >= 64 * W * 2) W *= 2;
@@ -925,9 +918,11 @@ cudaError_t launch_long(const RowArgs& a, int span, cudaStream_t s, int sms) {
     // but 148 x 8192 8.6 us with four against 4.0 with one: clusters start slowly.
     if (W == 8)
         while (C < 8 && a.V / (C * 2) >= 8192 && a.rows * C * 2 <= 4 * sms) C *= 2;
-    if (W == 1) return launch_long<T, K, 1, 4>(a, 1, s);
-    if (W == 2) return launch_long<T, K, 2, 1>(a, 1, s);
-    if (W == 4) return launch_long<T, K, 4, 1>(a, 1, s);
+    if constexpr (sizeof(K) == 4 || sizeof(T) == 4) {   // 16-bit rows that need 64-bit keys have over 8192 vectors: W = 8
+        if (W == 1) return launch_long<T, K, 1, 4>(a, 1, s);
+        if (W == 2) return launch_long<T, K, 2, 1>(a, 1, s);
+        if (W == 4) return launch_long<T, K, 4, 1>(a, 1, s);
+    }
     return launch_long<T, K, 8, 1>(a, C, s);
 }
 
@@ -936,24 +931,24 @@ cudaError_t launch_rows(const RowArgs& a, cudaStream_t s, int sms) {
     constexpr int N = VEC<T>;
     const int span = row_span<T>(a.x, a.stride, a.V);
     // Rows in registers as far as that is the faster way: without alternatives or with one up to 1024 elements; 16-bit logits
-    // with up to eight also (1024 bf16: 42 us for 2^25 logits, either way), with more up to 512 (512 with nine: 71 us, as long
-    // rows 90); fp32 logits, whose keys take 64 bits, up to 256 (257 with nine: 304 us, as long rows 162).
-    bool done = false;
+    // with up to eight also (1024 bf16: 38 us for 2^25 logits), with more up to 512 (512 with nine: 71 us, as long rows 90);
+    // fp32 logits, whose keys take 64 bits, up to 256 (257 with nine: 304 us, as long rows 162).
+    bool done;
     if (a.topk == 0) {
-        if (span <= N) { launch_lanes<T, 1, N, 0>(a, s); done = true; }
-        else if (span <= 16) { launch_lanes<T, 1, 16, 0>(a, s); done = true; }
-        else if (span <= 64) { launch_lanes<T, 4, 16, 0>(a, s); done = true; }
-        else done = launch_lanes<T, 32, 0>(a, span, s);
+        if (span <= N) done = launch_fit<T, 1, 1, N, 0>(a, span, s);
+        else if (span <= 16) done = launch_fit<T, 1, 1, 16, 0>(a, span, s);
+        else if (span <= 64) done = launch_fit<T, 4, 4, 16, 0>(a, span, s);
+        else done = launch_fit<T, 4, 32, 32, 0>(a, span, s);
     } else if (a.topk == 1) {
-        if (span <= N) { launch_lanes<T, 1, N, 1>(a, s); done = true; }
-        else done = launch_lanes<T, 32, 1>(a, span, s);
+        if (span <= N) done = launch_fit<T, 1, 1, N, 1>(a, span, s);
+        else done = launch_fit<T, 1, 32, 32, 1>(a, span, s);
     } else if (a.topk <= 8) {
-        if (span <= N) { launch_lanes<T, 1, N, N>(a, s); done = true; }
-        else if (span <= 8) { launch_lanes<T, 1, 8, 8>(a, s); done = true; }
-        else if (span <= 16) { launch_lanes<T, 1, 16, 8>(a, s); done = true; }
-        else if (span <= (sizeof(T) == 2 ? 1024 : 256)) done = a.topk <= 4 ? launch_sorted<T, 4>(a, span, s) : launch_sorted<T, 8>(a, span, s);
-    } else if (sizeof(T) == 2 || span <= 256) {
-        done = launch_lanes<T, 16, 16>(a, span, s);
+        if (span <= N) done = launch_fit<T, 1, 1, N, N>(a, span, s);
+        else if (N < 8 && span <= 8) done = launch_fit<T, 1, 1, 8, 8>(a, span, s);
+        else if (span <= 16) done = launch_fit<T, 1, 1, 16, 8>(a, span, s);
+        else done = a.topk <= 4 ? launch_sorted<T, 4>(a, span, s) : launch_sorted<T, 8>(a, span, s);
+    } else {
+        done = launch_fit<T, 1, sizeof(T) == 2 ? 32 : 16, 16, 16>(a, span, s);
     }
     if (!done) {
         typedef typename std::conditional<sizeof(T) == 2, uint32_t, unsigned long long>::type K;
