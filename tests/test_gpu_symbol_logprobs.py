@@ -82,7 +82,9 @@ def reference(x, s, topk):
 
 
 def close(got, want, atol, rtol=2 * U):
-    got, want = got.double().cpu().numpy(), np.asarray(want)
+    got, want = got.double().cpu().numpy(), np.asarray(want, np.float64)
+    with np.errstate(over="ignore"):   # outputs are 32 bits: a difference of the two largest logits is infinite there
+        want = np.where(np.isinf(want.astype(np.float32)), np.copysign(np.inf, want), want)
     same = (got == want) | (np.isnan(got) & np.isnan(want))
     with np.errstate(invalid="ignore"):
         ok = same | (np.abs(got - want) <= atol + rtol * np.abs(want))
@@ -175,6 +177,27 @@ def test_alternatives_of_hard_rows(kind, v, cuda_device):
     x = x.repeat(3, 1)
     s = torch.tensor([0, v // 2, v - 1])
     check_forward(x.cuda(), s.cuda(), x.double().numpy(), s.numpy(), 32)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("v", [4, 8, 60, 256, 700, 3000])
+def test_subnormal_and_extreme_logits(v, dtype, cuda_device):
+    """Subnormal numbers keep their order among themselves and around the two zeros; the largest finite values stand."""
+    info = torch.finfo(DT[dtype])
+    gen = torch.Generator().manual_seed(v)
+    tiny = info.smallest_normal * info.eps   # the smallest subnormal
+    x = torch.zeros(6, v, dtype=DT[dtype])
+    x[0] = (torch.randint(-3, 4, (v,), generator=gen).double() * tiny).to(DT[dtype])
+    x[1] = torch.where(torch.arange(v) % 2 == 0, -0.0, 0.0)
+    x[1, v // 2] = tiny
+    x[2] = info.max * (torch.randint(0, 2, (v,), generator=gen) * 2 - 1)
+    x[3] = info.min
+    x[3, v - 1] = info.max
+    x[4] = torch.linspace(-60, 60, v).to(DT[dtype])
+    x[5, 1:] = -info.max
+    s = torch.tensor([0, 1, v - 1, v - 1, v // 2, 0])
+    for topk in sorted({1, 2, min(v, 8), min(v, 20)}):
+        check_forward(x.cuda(), s.cuda(), x.double().numpy(), s.numpy(), topk)
 
 
 def grad_reference(x, s, dl, dh):
