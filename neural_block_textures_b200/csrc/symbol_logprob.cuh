@@ -9,7 +9,7 @@
 // a NaN or +inf gives NaN.
 //
 // Exponents (Scale below): e^d = 2^y with y = x L - mL in one fused multiply-add, L = log2 e and mL = m L rounded. All
-// y of a row are off by the same e0 = mL - m L, which is known exactly and put back where the row is finished, so the only
+// y of a row are off by the same mL - m L, which is known exactly and put back where the row is finished, so the only
 // rounding is y's own. y is clamped at kYLow, where 2^y is 0 in 32 bits: -inf and the type's lowest value then add 0 to u,
 // not 0 * inf; the clamp passes NaN on. Two elements share an instruction (fma.f32x2) where they can: the kernels are
 // bound by instruction issue and by the exponential unit (16 a clock and SM) before they are bound by memory.
@@ -146,35 +146,53 @@ __device__ __forceinline__ float max_of(const uint4 (&a)[C]) {
 
 // ------------------------------------------------------------------------------------------------------ a row's sums
 
-// The factors of one maximum (or lse) m: y = x L + b. Where |m| is 2^120 or more m L could overflow, and no logit but m's
-// equals can be within 2^90 of it: L = 2^-10 is exact there and keeps e^d right (1 or 0).
+// The exponents of one maximum (or lse) m. Near zero (|m| < 4096) y = x L + b, off by `off` = mL - m L for every x (at most
+// 2^-11, so that 2^off is 1 + off ln 2); far from it, where that would grow, y = (x - m) L, an instruction more and exact
+// where it counts.
 struct Scale {
-    float L, b;
-    __device__ __forceinline__ explicit Scale(float m) {
-        L = fabsf(m) >= 1.329227996e36f ? 0.0009765625f : kLog2e;
-        b = -(m * L);
+    float m, b, off;
+    bool far;
+    __device__ __forceinline__ explicit Scale(float at) : m(at) {
+        far = !(fabsf(at) < 4096.0f);
+        b = -(at * kLog2e);
+        off = far ? 0.0f : -fmaf(at, kLog2e, b);
     }
-    __device__ __forceinline__ float off(float m) const { return -fmaf(m, L, b); }   // mL - m L
 };
 struct Sums { float m, s, u; };
 
-// Adds N elements (even) with the factors c to s and u (pairs of partial sums).
-template <int N>
-__device__ __forceinline__ void add_exp(const float (&x)[N], const Scale& c, float2& s, float2& u) {
-    const float2 L = make_float2(c.L, c.L), b = make_float2(c.b, c.b);
+template <bool FAR>
+__device__ __forceinline__ float2 exponents(float x0, float x1, const Scale& c) {
+    const float2 x = make_float2(x0, x1), L = make_float2(kLog2e, kLog2e);
+    float2 y;
+    if constexpr (FAR) y = __fmul2_rn(__fadd2_rn(x, make_float2(-c.m, -c.m)), L);
+    else y = __ffma2_rn(x, L, make_float2(c.b, c.b));
+    y.x = max_nan(y.x, kYLow); y.y = max_nan(y.y, kYLow);
+    return y;
+}
+// Adds the elements of C vectors with the exponents of c to s and u (pairs of partial sums).
+template <bool FAR, class T, int C>
+__device__ __forceinline__ void add_exp(const uint4 (&raw)[C], const Scale& c, float2& s, float2& u) {
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-        float2 y = __ffma2_rn(make_float2(x[i], x[i + 1]), L, b);
-        y.x = max_nan(y.x, kYLow); y.y = max_nan(y.y, kYLow);
-        const float2 e = make_float2(exp2_of(y.x), exp2_of(y.y));
-        s = __fadd2_rn(s, e);
-        u = __ffma2_rn(e, y, u);
+    for (int k = 0; k < C; k++) {
+        float x[VEC<T>];
+        expand<T>(raw[k], x);
+#pragma unroll
+        for (int i = 0; i < VEC<T>; i += 2) {
+            const float2 y = exponents<FAR>(x[i], x[i + 1], c);
+            const float2 e = make_float2(exp2_of(y.x), exp2_of(y.y));
+            s = __fadd2_rn(s, e);
+            u = __ffma2_rn(e, y, u);
+        }
     }
 }
+template <class T, int C>
+__device__ __forceinline__ void add_exp(const uint4 (&raw)[C], const Scale& c, float2& s, float2& u) {
+    if (c.far) add_exp<true, T>(raw, c, s, u);
+    else add_exp<false, T>(raw, c, s, u);
+}
 // s and u of one maximum, without the common offset and in natural units.
-__device__ __forceinline__ Sums sums_of(float m, const Scale& c, float s, float u) {
-    const float off = c.off(m);
-    return Sums{m, fmaf(s, off * kLn2, s), kLn2 * fmaf(s, off, u)};
+__device__ __forceinline__ Sums sums_of(const Scale& c, float s, float u) {
+    return Sums{c.m, fmaf(s, c.off * kLn2, s), kLn2 * fmaf(s, c.off, u)};
 }
 // Joins two partial rows: s and u are relative to m.
 __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
@@ -428,16 +446,11 @@ __device__ __forceinline__ void rate_row(const RowArgs& a, const RowIn<T, E / VE
     for (int o = G / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
     const Scale sc(m);
     float2 s2 = make_float2(0.0f, 0.0f), u2 = s2;
-#pragma unroll
-    for (int c = 0; c < C; c++) {
-        float x[N];
-        expand<T>(raw[c], x);
-        add_exp(x, sc, s2, u2);
-    }
+    add_exp<T>(raw, sc, s2, u2);
     float2 q2 = make_float2(s2.x + s2.y, u2.x + u2.y);
 #pragma unroll
     for (int o = G / 2; o; o >>= 1) q2 = __fadd2_rn(q2, make_float2(__shfl_xor_sync(kFull, q2.x, o), __shfl_xor_sync(kFull, q2.y, o)));
-    const RowOut o = finish_row(sums_of(m, sc, q2.x, q2.y));
+    const RowOut o = finish_row(sums_of(sc, q2.x, q2.y));
     if (live && lane == 0) {
         if constexpr (G == 1 && E <= 8) {   // the logit is at hand
             float xt = NAN;
@@ -585,10 +598,10 @@ __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, i
     const int rounds = (end - first + U * kThreads - 1) / (U * kThreads);
     int lg = 0;   // rounds of a slot, as a power of two
     while ((rounds - 1) >> lg >= kSlots) lg++;
-    float m = kLowest, mine = kNegInf;   // the running maximum; this slot's (-inf: no logit)
+    float mine = kNegInf;                // this slot's largest logit (-inf: none)
     float most = kNegInf;                // this thread's largest logit
     int round = 0;
-    Scale sc(m);
+    Scale sc(kLowest);                   // of the running maximum
     float2 s2 = make_float2(0.0f, 0.0f), u2 = s2;
     for (int c = first + tid; c < end; c += U * kThreads) {
         uint4 raw[U];
@@ -603,22 +616,16 @@ __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, i
                 mine = kNegInf;
             }
         }
-        if (gm > m) {   // y of what is summed so far moves by the difference of the b
+        if (gm > sc.m) {   // y of what is summed so far moves
             const Scale to(gm);
-            const float y = max_nan(to.b - sc.b, kYLow), e = exp2_of(y);
+            const float y = max_nan(fmaf(sc.m - gm, kLog2e, sc.off - to.off), kYLow), e = exp2_of(y);
             u2.x = (u2.x + s2.x * y) * e; u2.y = (u2.y + s2.y * y) * e;
             s2.x *= e; s2.y *= e;
-            m = gm;
             sc = to;
         }
-#pragma unroll
-        for (int k = 0; k < U; k++) {
-            float v[N];
-            expand<T>(raw[k], v);
-            add_exp(v, sc, s2, u2);
-        }
+        add_exp<T>(raw, sc, s2, u2);
     }
-    Sums q = sums_of(m, sc, s2.x + s2.y, u2.x + u2.y);
+    Sums q = sums_of(sc, s2.x + s2.y, u2.x + u2.y);
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         const Sums p{__shfl_xor_sync(kFull, q.m, o), __shfl_xor_sync(kFull, q.s, o), __shfl_xor_sync(kFull, q.u, o)};
@@ -776,20 +783,27 @@ __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, i
 
 // -------------------------------------------------------------------------------------------------------- gradient
 
-// A thread takes M vectors of a row: 2^lg threads share a row (256 >> lg rows a CTA), or a row takes `chunks` CTAs. Four
-// vectors share the row's scalars and keep enough loads in flight; up to eight vectors a row take one each, so that short
-// rows' stores stay whole. Bound by memory: 4001 x 16411 fp32 with entropy 88 us (6.0 TB/s, at 92 % of a copy's rate), 2^18
-// x 256 bf16 49 us (5.6), 2^20 x 4 fp32 8.0 us (5.4, launch included).
-template <class T, int M, bool ENTROPY>
+// A thread takes M vectors of a row at a time. Rows of up to 128 vectors: 2^lg threads of a warp share a row. Longer ones
+// (CTA): a CTA has one row's part, `chunks` CTAs a row, or the whole row where the gradient is written over the logits.
+// Four vectors share the row's scalars and keep enough loads in flight; up to eight vectors a row take one each, so that
+// short rows' stores stay whole. Bound by memory: 4001 x 16411 fp32 with entropy 88 us (6.0 TB/s, at 92 % of a copy's rate),
+// 2^18 x 256 bf16 49 us (5.6), 2^20 x 4 fp32 8.0 us (5.4, launch included).
+//
+// The lse is rounded to 32 bits, which is off by 2^-24 of its size: p would be off by that, and wholly wrong where all of a
+// row is masked by a large finite value (p = 1 everywhere for a row of -1e9). So rows whose lse is 256 or more in size are
+// summed up once more, relative to that lse, and p is divided by the sum. All of a row's threads that may have written
+// parts of it in place wait for that sum.
+template <class T, int M, bool ENTROPY, bool CTA>
 __global__ void __launch_bounds__(256) k_logprobs_grad(const GradArgs a, int lg) {
     constexpr int N = VEC<T>;
-    const int group = 1 << lg;
-    const long long r = a.chunks > 1 ? (long long)(blockIdx.x / (unsigned)a.chunks) : (long long)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
-    const int c0 = (a.chunks > 1 ? (int)(blockIdx.x % (unsigned)a.chunks) * M * 256 : 0) + (threadIdx.x & (group - 1));
+    const int group = CTA ? (int)blockDim.x : 1 << lg;
+    const long long r = CTA ? (long long)(blockIdx.x / (unsigned)a.chunks) : (long long)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
+    const int lane = CTA ? (int)threadIdx.x : threadIdx.x & (group - 1);
     if (r >= a.rows) return;
     const T* row = static_cast<const T*>(a.x) + r * a.stride;
     T* out = static_cast<T*>(a.dx) + r * a.dx_stride;
-    const int shift = row_shift(row), V = a.V;
+    const int shift = row_shift(row), V = a.V, nvec = (V + shift + N - 1) / N;
+    int c0 = lane + (CTA ? (int)(blockIdx.x % (unsigned)a.chunks) * M * group : 0);
     uint4 raw[M];
 #pragma unroll
     for (int k = 0; k < M; k++) raw[k] = load_vec<false>(row, (c0 + k * group) * N - shift, V);
@@ -799,60 +813,93 @@ __global__ void __launch_bounds__(256) k_logprobs_grad(const GradArgs a, int lg)
     if (t >= V) dl = NAN;
     const bool empty = lse == kNegInf;
     const Scale sc(empty ? 0.0f : lse);
-    const float off = sc.off(empty ? 0.0f : lse);   // p = 2^(y + off), x - lse = (y + off) ln 2
-    const float p0 = -fmaf(off, kLn2, 1.0f);        // -2^off
+    float p0 = -fmaf(sc.off, kLn2, 1.0f);   // p = -p0 2^y (2^off, or 1 / sum)
+    float shift_nat = sc.off * kLn2;        // log p = y ln 2 + shift_nat
+    if (!empty && fabsf(lse) >= 256.0f) {
+        float2 s2 = make_float2(0.0f, 0.0f), u2 = s2;
+        const int step = CTA ? group : min(group, 32);
+        for (int c = lane; c < nvec; c += step) {
+            const uint4 one[1] = {load_vec<false>(row, c * N - shift, V)};
+            add_exp<T>(one, sc, s2, u2);
+        }
+        float s = s2.x + s2.y;
+        if constexpr (CTA) {
+            __shared__ float part[8];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
+            if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+            __syncthreads();
+            s = 0.0f;
+            for (int w = 0; w < group / 32; w++) s += part[w];
+        } else {
+            const unsigned mask = group == 32 ? kFull : ((1u << group) - 1u) << ((threadIdx.x & 31) & ~(group - 1));
+            for (int o = group / 2; o; o >>= 1) s += __shfl_xor_sync(mask, s, o);
+        }
+        p0 = __fdividef(-1.0f, s);
+        shift_nat = -logf(s);
+    }
     float dh = 0.0f, base = dl;
     if constexpr (ENTROPY) {
         dh = a.dentropy[r * a.dentropy_stride];
-        base = fmaf(dh, fmaf(off, kLn2, a.entropy[r]), dl);
+        base = fmaf(dh, shift_nat + a.entropy[r], dl);
         dh *= kLn2;
     }
-    const float2 L2 = make_float2(sc.L, sc.L), b2 = make_float2(sc.b, sc.b), dh2 = make_float2(dh * p0, dh * p0), base2 = make_float2(base * p0, base * p0);
+    // the exponents of either kind of Scale without a choice per element: (x - 0) L + b or (x - m) L + 0
+    const float from = sc.far ? -sc.m : 0.0f, b = sc.far ? 0.0f : sc.b;
+    const float2 from2 = make_float2(from, from), b2 = make_float2(b, b), dh2 = make_float2(dh * p0, dh * p0), base2 = make_float2(base * p0, base * p0);
+    for (;;) {
 #pragma unroll
-    for (int k = 0; k < M; k++) {
-        const int j0 = (c0 + k * group) * N - shift;
-        if (j0 >= V) break;
-        float v[N];
-        expand<T>(raw[k], v);
+        for (int k = 0; k < M; k++) {
+            const int j0 = (c0 + k * group) * N - shift;
+            if (j0 >= V) break;
+            float v[N];
+            expand<T>(raw[k], v);
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            float2 y = __ffma2_rn(make_float2(v[i], v[i + 1]), L2, b2);
-            y.x = max_nan(y.x, kYLow); y.y = max_nan(y.y, kYLow);
-            const float2 p = make_float2(exp2_of(y.x), exp2_of(y.y));
-            const float2 g = ENTROPY ? __fmul2_rn(p, __ffma2_rn(dh2, y, base2)) : __fmul2_rn(p, base2);
-            v[i] = g.x; v[i + 1] = g.y;
-        }
-        if (t >= j0 && t < j0 + N) {
-#pragma unroll
-            for (int i = 0; i < N; i++)
-                if (j0 + i == t) v[i] += dl;
-        }
-        if (empty) {
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] = 0.0f;
-        }
-        uint4 w;
-        if constexpr (sizeof(T) == 4) w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-        else {
-            uint32_t h[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if constexpr (std::is_same_v<T, __half>) { const __half2 e = __floats2half2_rn(v[2 * i], v[2 * i + 1]); memcpy(&h[i], &e, 4); }
-                else { const __nv_bfloat162 e = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); memcpy(&h[i], &e, 4); }
+            for (int i = 0; i < N; i += 2) {
+                float2 y = __ffma2_rn(__fadd2_rn(make_float2(v[i], v[i + 1]), from2), make_float2(kLog2e, kLog2e), b2);
+                y.x = max_nan(y.x, kYLow); y.y = max_nan(y.y, kYLow);
+                const float2 p = make_float2(exp2_of(y.x), exp2_of(y.y));
+                const float2 g = ENTROPY ? __fmul2_rn(p, __ffma2_rn(dh2, y, base2)) : __fmul2_rn(p, base2);
+                v[i] = g.x; v[i + 1] = g.y;
             }
-            w = make_uint4(h[0], h[1], h[2], h[3]);
-        }
-        if (j0 >= 0 && j0 + N <= V && (reinterpret_cast<uintptr_t>(out + j0) & 15) == 0) {
-            __stcs(reinterpret_cast<uint4*>(out + j0), w);
-        } else {
-            const uint32_t h[4] = {w.x, w.y, w.z, w.w};
+            if (t >= j0 && t < j0 + N) {
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                if (j0 + i < 0 || j0 + i >= V) continue;
-                if constexpr (sizeof(T) == 4) out[j0 + i] = v[i];
-                else { const unsigned short e = (unsigned short)(h[i / 2] >> (16 * (i % 2))); memcpy(out + j0 + i, &e, 2); }
+                for (int i = 0; i < N; i++)
+                    if (j0 + i == t) v[i] += dl;
+            }
+            if (empty) {
+#pragma unroll
+                for (int i = 0; i < N; i++) v[i] = 0.0f;
+            }
+            uint4 w;
+            if constexpr (sizeof(T) == 4) w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            else {
+                uint32_t h[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if constexpr (std::is_same_v<T, __half>) { const __half2 e = __floats2half2_rn(v[2 * i], v[2 * i + 1]); memcpy(&h[i], &e, 4); }
+                    else { const __nv_bfloat162 e = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); memcpy(&h[i], &e, 4); }
+                }
+                w = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+            if (j0 >= 0 && j0 + N <= V && (reinterpret_cast<uintptr_t>(out + j0) & 15) == 0) {
+                __stcs(reinterpret_cast<uint4*>(out + j0), w);
+            } else {
+                const uint32_t h[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    if (j0 + i < 0 || j0 + i >= V) continue;
+                    if constexpr (sizeof(T) == 4) out[j0 + i] = v[i];
+                    else { const unsigned short e = (unsigned short)(h[i / 2] >> (16 * (i % 2))); memcpy(out + j0 + i, &e, 2); }
+                }
             }
         }
+        if constexpr (!CTA) return;
+        if (a.chunks > 1) return;
+        c0 += M * group;   // a CTA with a whole row goes on
+        if (c0 - lane >= nvec) return;
+#pragma unroll
+        for (int k = 0; k < M; k++) raw[k] = load_vec<false>(row, (c0 + k * group) * N - shift, V);
     }
 }
 
@@ -965,12 +1012,15 @@ cudaError_t launch_grad(GradArgs a, cudaStream_t s) {
     a.chunks = 1;
     if (nvec <= 8) {
         while ((1 << lg) < nvec) lg++;
-        k_logprobs_grad<T, 1, ENTROPY><<<(unsigned)ceil_div(a.rows, 256 >> lg), 256, 0, s>>>(a, lg);
-    } else {
+        k_logprobs_grad<T, 1, ENTROPY, false><<<(unsigned)ceil_div(a.rows, 256 >> lg), 256, 0, s>>>(a, lg);
+    } else if (nvec <= 128) {
         lg = 1;
-        while (lg < 8 && (4 << lg) < nvec) lg++;
-        if (lg == 8) a.chunks = (int)ceil_div(nvec, 1024);
-        k_logprobs_grad<T, 4, ENTROPY><<<(unsigned)(a.chunks > 1 ? a.rows * a.chunks : ceil_div(a.rows, 256 >> lg)), 256, 0, s>>>(a, lg);
+        while ((4 << lg) < nvec) lg++;
+        k_logprobs_grad<T, 4, ENTROPY, false><<<(unsigned)ceil_div(a.rows, 256 >> lg), 256, 0, s>>>(a, lg);
+    } else {
+        const int threads = nvec <= 256 ? 64 : nvec <= 512 ? 128 : 256;
+        if (a.dx != a.x) a.chunks = (int)ceil_div(nvec, 4 * threads);
+        k_logprobs_grad<T, 4, ENTROPY, true><<<(unsigned)(a.rows * a.chunks), threads, 0, s>>>(a, 0);
     }
     return cudaGetLastError();
 }

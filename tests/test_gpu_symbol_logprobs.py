@@ -207,14 +207,19 @@ def grad_reference(x, s, dl, dh):
     for r in range(n):
         if np.isneginf(lse[r]):
             continue
-        lp = x[r] - lse[r]
+        m = x[r].max()
+        lp = x[r] - m - math.log(math.fsum(np.exp(x[r] - m)))
         p = np.exp(lp)
         lp = np.where(p > 0, lp, 0.0)
         a = dl[r] if s[r] >= 0 else 0.0
         dx[r] = -p * (a + dh[r] * (lp + ent[r]))
-        # roundings: the exponent (2^-23 of its size and of lse's), the exponential, the factor, the product
-        scale[r] = p * (abs(a) + abs(dh[r]) * (np.abs(lp) + ent[r] + 1)) * (8 + 4 * np.abs(lp) + 4 * abs(lse[r])) * U
+        # roundings: the exponent (2^-23 of its size and of lse's), the exponential, the factor, the product; a large lse
+        # (256 or more) is replaced by a new sum of the row, off by tol(v)
+        size = 4 * abs(lse[r]) if abs(lse[r]) < 256 else 2 * tol(v) / U
+        scale[r] = p * (abs(a) + abs(dh[r]) * (np.abs(lp) + ent[r] + 1)) * (8 + 4 * np.abs(lp) + size) * U
         scale[r] += p * abs(dh[r]) * 2 * tol(v) * (1 + math.log(v))
+        # probabilities below the smallest normal number are flushed to zero
+        scale[r] += 2.0 ** -126 * (abs(a) + abs(dh[r]) * (np.abs(lp) + ent[r] + 1))
         if s[r] >= 0:
             dx[r, s[r]] += a
             scale[r, s[r]] += 2 * U * abs(a)
@@ -229,7 +234,7 @@ def check_grad(x, s, x64, s64, dl, dh, dtype, **kw):
     want, scale = grad_reference(x64, s64, full(dl), full(dh))
     info = torch.finfo(DT[dtype])
     err = np.abs(got.double().cpu().numpy() - want)
-    bad = err > scale + np.abs(want) * info.eps / 2 + info.smallest_normal * info.eps
+    bad = ~(err <= scale + np.abs(want) * info.eps / 2 + info.smallest_normal * info.eps)
     assert not bad.any(), (err[bad].max(), np.argwhere(bad)[:4])
     assert got.dtype == DT[dtype]
     return got
@@ -258,6 +263,37 @@ def test_gradient_strides_and_in_place(v, stride, offset, dtype, cuda_device):
     r = symbol_logprobs(x, s)
     out = symbol_logprobs_grad(x, s, r.lse, r.entropy, -1.0, 0.1, out=x)
     assert out.data_ptr() == x.data_ptr() and torch.equal(x, want)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("v", [2, 4, 7, 30, 250, 1000, 1100, 2100, 4200, 9000, 40000])
+def test_gradient_of_rows_far_from_zero(v, dtype, cuda_device):
+    """A softmax does not change with a shift of its logits: rows around a large value, rows wholly masked by large finite
+    values (the type's lowest, -1e9 or what the type has of it), one logit beside them; in place gives the same."""
+    info = torch.finfo(DT[dtype])
+    gen = torch.Generator().manual_seed(v)
+    base = torch.randn(9, v, generator=gen) * 2
+    x = base.clone()
+    x[1] = info.min
+    x[2] = max(-1e9, info.min)
+    x[3] = info.max
+    x[4] = x[4] * 8 + 3000
+    x[5] = x[5] * 8 - 3000
+    x[6] = info.min
+    x[6, v // 2] = 1.0
+    x[7] = max(-1e9, info.min)
+    x[7, v - 1] = 2.0
+    x[8] = x[8] + 300
+    x = x.to(DT[dtype])
+    s = torch.randint(0, v, (9,), generator=gen)
+    x64, s64, x, s = x.double().numpy(), s.numpy(), x.cuda(), s.cuda()
+    dl, dh = torch.randn(9, generator=gen).cuda(), torch.randn(9, generator=gen).cuda()
+    check_grad(x, s, x64, s64, dl, None, dtype)
+    want = check_grad(x, s, x64, s64, dl, dh, dtype)
+    check_forward(x, s, x64, s64, min(v, 5))   # its sums may be rounded otherwise than without alternatives
+    r = symbol_logprobs(x, s)
+    symbol_logprobs_grad(x, s, r.lse, r.entropy, dl, dh, out=x)
+    assert torch.equal(x, want)
 
 
 def test_gradient_against_differences(cuda_device):
