@@ -783,18 +783,45 @@ __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, i
 
 // -------------------------------------------------------------------------------------------------------- gradient
 
+// The sum of a row's exponentials relative to its lse, by the row's `group` threads (at most a warp's, or a CTA).
+template <class T, bool CTA>
+__device__ __forceinline__ float row_sum(const T* row, int V, int shift, int lane, int group, float lse) {
+    constexpr int N = VEC<T>;
+    const Scale sc(lse);
+    float2 s2 = make_float2(0.0f, 0.0f), u2 = s2;
+    for (int c = lane; c * N - shift < V; c += group) {
+        const uint4 one[1] = {load_vec<false>(row, c * N - shift, V)};
+        add_exp<T>(one, sc, s2, u2);
+    }
+    float s = s2.x + s2.y;
+    if constexpr (CTA) {
+        __shared__ float part[8];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+        __syncthreads();
+        s = 0.0f;
+        for (int w = 0; w < group / 32; w++) s += part[w];
+    } else {
+        const unsigned mask = group == 32 ? kFull : ((1u << group) - 1u) << ((threadIdx.x & 31) & ~(group - 1));
+        for (int o = group / 2; o; o >>= 1) s += __shfl_xor_sync(mask, s, o);
+    }
+    return s;
+}
+
 // A thread takes M vectors of a row at a time. Rows of up to 128 vectors: 2^lg threads of a warp share a row. Longer ones
 // (CTA): a CTA has one row's part, `chunks` CTAs a row, or the whole row where the gradient is written over the logits.
 // Four vectors share the row's scalars and keep enough loads in flight; up to eight vectors a row take one each, so that
-// short rows' stores stay whole. Bound by memory: 4001 x 16411 fp32 with entropy 88 us (6.0 TB/s, at 92 % of a copy's rate),
-// 2^18 x 256 bf16 49 us (5.6), 2^20 x 4 fp32 8.0 us (5.4, launch included).
+// short rows' stores stay whole. Bound by memory: 4001 x 16411 fp32 with entropy 90 us (5.8 TB/s, 89 % of a copy's rate), 2^18
+// x 256 bf16 52 us (5.3), 2^20 x 4 fp32 7.9 us (5.4, launch included); the launch bounds hold the registers that the second
+// sum (below) would take (without them 8.9, 55 and 91 us; as a function of its own 8.0, 56, 90).
 //
 // The lse is rounded to 32 bits, which is off by 2^-24 of its size: p would be off by that, and wholly wrong where all of a
 // row is masked by a large finite value (p = 1 everywhere for a row of -1e9). So rows whose lse is 256 or more in size are
 // summed up once more, relative to that lse, and p is divided by the sum. All of a row's threads that may have written
 // parts of it in place wait for that sum.
 template <class T, int M, bool ENTROPY, bool CTA>
-__global__ void __launch_bounds__(256) k_logprobs_grad(const GradArgs a, int lg) {
+__global__ void __launch_bounds__(256, M == 1 ? 8 : 5) k_logprobs_grad(const GradArgs a, int lg) {
     constexpr int N = VEC<T>;
     const int group = CTA ? (int)blockDim.x : 1 << lg;
     const long long r = CTA ? (long long)(blockIdx.x / (unsigned)a.chunks) : (long long)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
@@ -816,25 +843,7 @@ __global__ void __launch_bounds__(256) k_logprobs_grad(const GradArgs a, int lg)
     float p0 = -fmaf(sc.off, kLn2, 1.0f);   // p = -p0 2^y (2^off, or 1 / sum)
     float shift_nat = sc.off * kLn2;        // log p = y ln 2 + shift_nat
     if (!empty && fabsf(lse) >= 256.0f) {
-        float2 s2 = make_float2(0.0f, 0.0f), u2 = s2;
-        const int step = CTA ? group : min(group, 32);
-        for (int c = lane; c < nvec; c += step) {
-            const uint4 one[1] = {load_vec<false>(row, c * N - shift, V)};
-            add_exp<T>(one, sc, s2, u2);
-        }
-        float s = s2.x + s2.y;
-        if constexpr (CTA) {
-            __shared__ float part[8];
-#pragma unroll
-            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
-            if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
-            __syncthreads();
-            s = 0.0f;
-            for (int w = 0; w < group / 32; w++) s += part[w];
-        } else {
-            const unsigned mask = group == 32 ? kFull : ((1u << group) - 1u) << ((threadIdx.x & 31) & ~(group - 1));
-            for (int o = group / 2; o; o >>= 1) s += __shfl_xor_sync(mask, s, o);
-        }
+        const float s = row_sum<T, CTA>(row, V, shift, lane, group, lse);
         p0 = __fdividef(-1.0f, s);
         shift_nat = -logf(s);
     }
