@@ -526,7 +526,7 @@ __device__ __forceinline__ void rate_row(const RowArgs& a, const RowIn<T, E / VE
     }
 }
 
-// Measured: 2^18 x 256 bf16 29 us without alternatives (5.2 TB/s of the 6.5 that a copy reaches), 36 with one, 72 with eight
+// Measured: 2^18 x 256 bf16 29 us without alternatives (5.2 TB/s of the 6.5 that a copy reaches), 37 with one, 74 with eight
 // (the minima and maxima of the sorts, on the half-rate logic unit, near 80 % busy); 2^15 x 1024 fp32 at the memory's rate; 2^20 x 4
 // fp32 9.2 and, with two alternatives, 12.4 us (instruction issue: the row's end is paid by every lane).
 // One group of rows to a CTA. (CTAs that stay and fetch the next rows ahead were slower on short rows: 17 against 15 us for
