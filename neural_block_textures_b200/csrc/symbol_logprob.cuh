@@ -190,9 +190,11 @@ __device__ __forceinline__ void add_exp(const uint4 (&raw)[C], const Scale& c, f
     if (c.far) add_exp<true, T>(raw, c, s, u);
     else add_exp<false, T>(raw, c, s, u);
 }
-// s and u of one maximum, without the common offset and in natural units.
+// s and u of one maximum, without the common offset and in natural units: the true exponents are y + off, so
+// sum e^d = 2^off s and sum e^d d = 2^off ln 2 (u + off s), both with 2^off = 1 + off ln 2 (off^2 is below 2^-22).
 __device__ __forceinline__ Sums sums_of(const Scale& c, float s, float u) {
-    return Sums{c.m, fmaf(s, c.off * kLn2, s), kLn2 * fmaf(s, c.off, u)};
+    const float grow = c.off * kLn2, t = kLn2 * fmaf(s, c.off, u);
+    return Sums{c.m, fmaf(s, grow, s), fmaf(t, grow, t)};
 }
 // Joins two partial rows: s and u are relative to m.
 __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {

@@ -448,3 +448,41 @@ def test_rows_behind_32_bits(cuda_device):
     want = symbol_logprobs_grad(tail.cuda(), s[n - 8:].cuda(), r.lse[n - 8:], r.entropy[n - 8:], -1.0)
     symbol_logprobs_grad(x, s.cuda(), r.lse, r.entropy, -1.0, out=x)
     assert torch.equal(x[n - 8:], want)
+
+
+def entropy_bound(x, v, long_row):
+    """What the entropy of one row may be off by. s sums e^d and u sums e^d d (one sign each, so nothing cancels): every
+    term is off by its exponential's 4 U and its exponent's 2.5 U |d| (a constant, a difference and a product rounded),
+    every sum and join by the roundings counted in `sums`; log s by two units, the quotient by four, their difference by
+    one, the offset of the exponents by 2 U. Lanes add at most 32 pairs one after another and join 6 times; a thread of a
+    long row adds 16 pairs and is moved to a new maximum (12 roundings) a round, and the parts join 11 times."""
+    d = x[x > -np.inf] - x.max()
+    p = np.exp(d)
+    p /= math.fsum(p)
+    e1, e2 = -math.fsum(p * d), math.fsum(p * d * d)
+    log_s = math.log(math.fsum(np.exp(d)))
+    rounds = min(8, -(-v // (4 * 4 * 256)))   # few rows: threads of 4 vectors, up to 256 of them a CTA, then more rounds
+    sums = 28 * rounds + 12 * 11 if long_row else 40
+    rel_s = sums + 6 + 2.5 * e1
+    return U * (rel_s * (1 + e1) + (sums + 10) * e1 + 2.5 * e2 + 2 * log_s + 4 * e1 + (log_s + e1))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("v", [3, 4, 11, 16, 60, 250, 256, 700, 1000, 1025, 4099, 9000, 65536])
+def test_entropy_of_rows_around_a_value(v, dtype, cuda_device):
+    """Logits of an ordinary spread around values up to where the exponents change their form: the entropy does not depend
+    on the value, and the gradient's entropy term, which reads it, neither."""
+    centres = [0, 3, 30, -100, 300, -300, 1000, -1000, 3000, -3000, 4080, -4080]
+    gen = torch.Generator().manual_seed(v)
+    x = (torch.randn(len(centres), v, generator=gen) * 2.5 + torch.tensor(centres)[:, None]).to(DT[dtype])
+    s = torch.randint(0, v, (len(centres),), generator=gen)
+    x64, s64 = x.double().numpy(), s.numpy()
+    _, want, _, _, _ = reference(x64, s64, 0)
+    limit = np.array([entropy_bound(row, v, v > 250) for row in x64])
+    for topk in sorted({0, 1, min(v, 3), min(v, 8), min(v, 20)}):
+        r = check_forward(x.cuda(), s.cuda(), x64, s64, topk)
+        err = np.abs(r.entropy.double().cpu().numpy() - want)
+        assert (err <= limit).all(), (topk, err, limit)
+    if v <= 4099:
+        dl, dh = torch.randn(len(centres), generator=gen).cuda(), torch.randn(len(centres), generator=gen).cuda()
+        check_grad(x.cuda(), s.cuda(), x64, s64, dl, dh, dtype)
