@@ -19,7 +19,10 @@ int dtype_code(at::ScalarType t) {
 int symbol_code(at::ScalarType t) {
     return t == at::kByte ? NTCB_SYM_U8 : t == at::kShort ? NTCB_SYM_I16 : t == at::kInt ? NTCB_SYM_I32 : t == at::kLong ? NTCB_SYM_I64 : -1;
 }
-bool plain(PyObject* o) { return THPVariable_Check(o) && THPVariable_Unpack(o).layout() == at::kStrided; }
+// A tensor whose memory holds its values as they are: a negated view (the imaginary part of a conjugate) holds their negatives.
+bool plain(PyObject* o) {
+    return THPVariable_Check(o) && THPVariable_Unpack(o).layout() == at::kStrided && !THPVariable_Unpack(o).is_neg();
+}
 
 // The description of plain logits [n, V] and symbols [n] on one CUDA device; false for anything else.
 bool describe(PyObject* logits, PyObject* symbols, ntcb_symbol_desc& d) {

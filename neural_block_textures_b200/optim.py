@@ -50,8 +50,8 @@ class AdamW:
                 raise TypeError("AdamW: parameters must be float32, float16 or bfloat16 tensors")
             if not p.is_cuda or p.device != self.params[0].device:
                 raise ValueError("AdamW: parameters must be on one CUDA device")
-            if not p.is_contiguous():
-                raise ValueError("AdamW: parameters must be contiguous")
+            if not p.is_contiguous() or p.is_neg():
+                raise ValueError("AdamW: parameters must be contiguous, and no negated views")
         spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("AdamW: two parameters share memory")
@@ -91,7 +91,7 @@ class AdamW:
 
     def _scalar(self, x: torch.Tensor, dtype: torch.dtype, name: str) -> tuple[int, int]:
         """(the host value's place holder, the device address) of a one-element device tensor."""
-        if x.dtype != dtype or x.numel() != 1 or x.device != self.device:
+        if x.dtype != dtype or x.numel() != 1 or x.device != self.device or x.is_neg():
             raise ValueError(f"AdamW.step: {name} as a tensor must be one {dtype} on {self.device}")
         return 1, x.data_ptr()
 

@@ -97,6 +97,8 @@ def symbol_logprobs(logits: torch.Tensor, symbols: torch.Tensor, topk: int = 0) 
         if r is not None:
             return SymbolLogprobs(*r)
     _, n, v, _ = _desc(logits, symbols, "symbol_logprobs")   # says what is wrong
+    if logits.is_neg():
+        return symbol_logprobs(logits.resolve_neg(), symbols, topk)
     if not 0 <= topk <= min(abi.MAX_TOPK, v):
         raise ValueError(f"symbol_logprobs: topk must be 0 .. {min(abi.MAX_TOPK, v)} here, not {topk}")
     raise ValueError("symbol_logprobs: logits and symbols must be strided tensors")
@@ -115,6 +117,13 @@ def symbol_logprobs_grad(logits: torch.Tensor, symbols: torch.Tensor, lse: torch
             return r
     d, n, v, device = _desc(logits, symbols, "symbol_logprobs_grad")
     dev = logits.device
+    if out is not None and out.is_neg():
+        raise ValueError("symbol_logprobs_grad: out must not be a negated view")
+    # the memory of a negated view holds the values' negatives
+    given = [x.resolve_neg() if isinstance(x, torch.Tensor) else x for x in (logits, lse, entropy, dlogp, dentropy)]
+    if given[0] is not logits:
+        return symbol_logprobs_grad(given[0], symbols, *given[1:], out=out)
+    _, lse, entropy, dlogp, dentropy = given
     if not isinstance(dlogp, torch.Tensor):
         dlogp = torch.full((1,), float(dlogp), device=dev).expand(n)
     if dentropy is not None and not isinstance(dentropy, torch.Tensor):

@@ -351,3 +351,17 @@ def test_a_symbol_model_is_trained(bits, cuda_device):
         if it == 1:
             moved = want.abs() > 1e-5
             assert (table + 0.05 * want.sign())[moved].abs().max() < 0.05 * 1e-2   # eps = 1e-8 over |g| > 1e-5: 0.1 %
+
+
+def test_negated_views_are_refused(cuda_device):
+    """Their memory holds the values' negatives: as a parameter, a gradient or a scalar they would act with the wrong sign."""
+    one = torch.randn(1, dtype=torch.complex64, device="cuda").conj().imag
+    assert one.is_neg() and one.is_contiguous()
+    with pytest.raises(ValueError, match="negated"):
+        AdamW([one])
+    p = torch.ones(1, device="cuda")
+    opt = AdamW([p])
+    for bad in (lambda: opt.step(1, 0.1, [one]), lambda: opt.step(1, one, [p.clone()]), lambda: opt.step(1, 0.1, [p.clone()], grad_scale=one)):
+        with pytest.raises(ValueError):
+            bad()
+    assert p.item() == 1.0

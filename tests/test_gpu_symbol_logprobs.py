@@ -486,3 +486,25 @@ def test_entropy_of_rows_around_a_value(v, dtype, cuda_device):
     if v <= 4099:
         dl, dh = torch.randn(len(centres), generator=gen).cuda(), torch.randn(len(centres), generator=gen).cuda()
         check_grad(x.cuda(), s.cuda(), x64, s64, dl, dh, dtype)
+
+
+def test_negated_views(cuda_device):
+    """The imaginary part of a conjugate is a view whose memory holds the values' negatives."""
+    negated = lambda n: torch.randn(n, dtype=torch.complex64, device="cuda").conj().imag
+    x, s, _, _ = make(9, 40, "f32", masks=False)
+    r = symbol_logprobs(x, s)
+    dl, dh, lse, h = negated(9), negated(9), negated(9), negated(9)
+    assert dl.is_neg() and dh.is_neg()
+    for args in ((r.lse, r.entropy, dl, None), (r.lse, r.entropy, dl, dh), (r.lse, h, dl, dh), (lse, r.entropy, -1.0, dh)):
+        got = symbol_logprobs_grad(x, s, *args)
+        assert torch.equal(got, symbol_logprobs_grad(x, s, *[a.clone() if isinstance(a, torch.Tensor) else a for a in args]))
+    column = torch.stack([torch.zeros(9, device="cuda"), -x[:, 0]], 1)   # one logit a row, two floats apart
+    one = torch.view_as_complex(column).conj().imag[:, None]
+    assert one.is_neg() and torch.equal(one, x[:, :1])
+    z = torch.zeros_like(s)
+    a, b = symbol_logprobs(one, z, topk=1), symbol_logprobs(x[:, :1], z, topk=1)
+    assert torch.equal(a.lse, b.lse) and torch.equal(a.logp, b.logp)
+    da, db = (symbol_logprobs_grad(y, z, a.lse, a.entropy, -1.0, 0.5) for y in (one, x[:, :1]))
+    assert torch.equal(da, db)
+    with pytest.raises(ValueError, match="negated"):
+        symbol_logprobs_grad(x[:, :1], z, a.lse, a.entropy, -1.0, out=one)
