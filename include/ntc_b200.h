@@ -399,7 +399,8 @@ int ntcb_symbol_logprobs_grad(const ntcb_symbol_desc* d, const void* logits, con
 
 /* AdamW over many tensors in one step: m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2 (g the gradient times
  * grad_scale), p = (1 - lr weight_decay) p - lr (m / (1 - b1^it)) / (sqrt(v / (1 - b2^it)) + eps), in 32 bits, the
- * parameters rounded to nearest where they are held in 16. With weight_decay 0 it is the trainer's own Adam.
+ * parameters rounded to nearest where they are held in 16. eps is 0 or a normal 32-bit number (1.18e-38 or more). With
+ * weight_decay 0 it is the trainer's own Adam.
  * A plan holds the tensors' sizes and types and a device table of the work, no pointer of the caller's; the moments are
  * the caller's buffer of ntcb_adamw_state_bytes bytes (256-byte aligned, zeroed before the first step).
  *

@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <new>
 #include <type_traits>
@@ -168,7 +169,8 @@ __device__ __forceinline__ void update2(const Scalars& c, float2& p, float2 g, f
         asm("sqrt.approx.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
         asm("sqrt.approx.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
     }
-    r = __ffma2_rn(r, both(c.inv), both(c.eps));   // between 2^-75 (or 0) and 2^65: its reciprocal needs no care for subnormals
+    r = __ffma2_rn(r, both(c.inv), both(c.eps));   // eps is 0 or normal and a root of v at least 2^-75, so r is 0 or normal: its
+    // reciprocal needs no care for subnormals
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r.x));
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r.y));
     p = __ffma2_rn(__fmul2_rn(m, both(-c.step)), r, __fmul2_rn(p, both(c.decay)));
@@ -548,6 +550,7 @@ int ntcb_adamw_step(const ntcb_adamw* a, void* const* params, const void* const*
     if (!(args->beta1 >= 0.0 && args->beta1 < 1.0 && args->beta2 >= 0.0 && args->beta2 < 1.0)) return refuse("a beta is outside [0, 1)");
     if (!(args->eps >= 0.0) || !(args->weight_decay >= 0.0) || std::isinf(args->eps) || std::isinf(args->weight_decay))
         return refuse("eps and weight_decay must be finite and not negative");
+    if (args->eps > 0.0 && args->eps < (double)FLT_MIN) return refuse("eps must be 0 or a normal 32-bit number (1.18e-38 or more)");
     if (!args->lr_dev && !(std::isfinite(args->lr) && args->lr >= 0.0)) return refuse("lr must be finite and not negative");
     if (!args->it_dev && (args->it < 1 || args->it > 0xffffffffll)) return refuse("it counts from 1 and stays below 2^32");
     for (int i = 0; i < n; i++) {

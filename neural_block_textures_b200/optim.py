@@ -43,6 +43,8 @@ class AdamW:
             raise ValueError("AdamW: betas must be in [0, 1)")
         if not eps >= 0.0 or not weight_decay >= 0.0:
             raise ValueError("AdamW: eps and weight_decay must not be negative")
+        if 0.0 < eps < torch.finfo(torch.float32).tiny:
+            raise ValueError("AdamW: eps must be 0 or at least 1.18e-38 (a normal 32-bit number)")
         if grad_dtype is not None and grad_dtype not in DTYPES:
             raise TypeError(f"AdamW: gradients must be float32, float16 or bfloat16, not {grad_dtype}")
         for p in self.params:

@@ -365,3 +365,20 @@ def test_negated_views_are_refused(cuda_device):
         with pytest.raises(ValueError):
             bad()
     assert p.item() == 1.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_smallest_eps(bits, cuda_device):
+    """The smallest eps that is taken leaves a parameter without a gradient where it was; a smaller one is refused, by the
+    step too."""
+    p = torch.ones(300, device="cuda")
+    opt = AdamW([p], state_bits=bits, eps=2.0 ** -126, weight_decay=0.0)
+    g = torch.zeros(300, device="cuda")
+    opt.step(1, 0.1, [g])
+    assert (p == 1).all()
+    g[0] = 1.0
+    opt.step(2, 0.1, [g])
+    assert p[0] < 1 and (p[1:] == 1).all()
+    opt.eps = 1e-40
+    with pytest.raises(RuntimeError, match="eps"):
+        opt.step(3, 0.1, [g])

@@ -151,3 +151,10 @@ def test_layout_matches_c_header(cls, name, tmp_path):
     assert int(out["sizeof"]) == C.sizeof(cls)
     for f in fields:
         assert getattr(cls, f).offset == int(out[f]), f
+
+
+def test_eps_below_the_normal_numbers_is_refused():
+    """Its reciprocal would be infinite and a zero gradient would leave NaN."""
+    for eps in (1e-40, 1.17e-38, 5e-324):
+        with pytest.raises(ValueError, match="eps"):
+            AdamW([torch.zeros(4, 8)], eps=eps)
