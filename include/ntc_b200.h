@@ -422,7 +422,8 @@ typedef struct ntcb_adamw_args {
     const float* grad_scale_dev;   /* multiplies grad_scale */
 } ntcb_adamw_args;
 /* Makes a plan for ntensors tensors of sizes[i] elements (0 allowed) of param_types[i] with gradients of grad_types[i].
- * Allocates the device table: not during a stream capture. NULL with a reason on failure. */
+ * Allocates the device table and waits until it is filled, so any stream may take the first step: not during a stream
+ * capture. NULL with a reason on failure. */
 ntcb_adamw* ntcb_adamw_create(int device, int ntensors, const long long* sizes, const int* param_types, const int* grad_types,
                               int state_bits, char* why, size_t why_cap);
 void ntcb_adamw_destroy(ntcb_adamw* a);

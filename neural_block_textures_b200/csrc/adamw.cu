@@ -507,7 +507,10 @@ ntcb_adamw* ntcb_adamw_create(int device, int ntensors, const long long* sizes, 
         a->device = scope.device;
         if (!table.empty()) {
             cudaError_t e = cudaMalloc(&a->chunks, table.size() * sizeof(Chunk));
-            if (e == cudaSuccess) e = cudaMemcpy(a->chunks, table.data(), table.size() * sizeof(Chunk), cudaMemcpyHostToDevice);
+            // A copy from pageable memory may return before it has reached the device, and streams that do not wait for the
+            // legacy stream may take the first step: the table must be there when the plan is.
+            if (e == cudaSuccess) e = cudaMemcpyAsync(a->chunks, table.data(), table.size() * sizeof(Chunk), cudaMemcpyHostToDevice, cudaStreamLegacy);
+            if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
             if (e != cudaSuccess) {
                 cudaGetLastError();
                 DeviceScope::fail("the table of work", e, why, why_cap);

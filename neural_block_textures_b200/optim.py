@@ -29,7 +29,8 @@ _pack_args = struct.Struct("6dqQ3Q").pack   # ntcb_adamw_args
 class AdamW:
     """params: contiguous float32, float16 or bfloat16 CUDA tensors on one device; kept, and written by step().
     grad_dtype: the gradients' type where it is not the parameter's. The state (`state`, one uint8 tensor) starts at
-    zero; it can be saved and restored with state_dict() / load_state_dict()."""
+    zero, set on the stream that is current here, which another stream's first step waits for as for any tensor's
+    contents; it can be saved and restored with state_dict() / load_state_dict()."""
 
     def __init__(self, params, state_bits: int = 32, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.01, seed: int = 0, grad_dtype: torch.dtype | None = None) -> None:

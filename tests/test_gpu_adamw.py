@@ -382,3 +382,21 @@ def test_smallest_eps(bits, cuda_device):
     opt.eps = 1e-40
     with pytest.raises(RuntimeError, match="eps"):
         opt.step(3, 0.1, [g])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_first_step_on_another_stream_at_once(bits, cuda_device):
+    """The plan's table is on the device when the plan is made: a stream that does not wait for the legacy one takes the
+    first step without a synchronisation in between (it waits for the tensors only)."""
+    for n in (300, 5_000_000):
+        p = torch.ones(n, device="cuda")
+        g = torch.full((n,), 0.5, device="cuda")
+        for _ in range(20):
+            stream = torch.cuda.Stream()
+            opt = AdamW([p], state_bits=bits, weight_decay=0.0)
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                p.fill_(1.0)
+                opt.step(1, 0.25, [g])
+                assert ((p - 0.75).abs() < 1e-5).all()
+            torch.cuda.current_stream().wait_stream(stream)
