@@ -426,7 +426,11 @@ typedef struct ntcb_adamw_args {
  * capture. NULL with a reason on failure. */
 ntcb_adamw* ntcb_adamw_create(int device, int ntensors, const long long* sizes, const int* param_types, const int* grad_types,
                               int state_bits, char* why, size_t why_cap);
+/* Frees the plan. A graph that captured a step has the addresses of the plan's table and of the buffers in it: the plan,
+ * the state, the parameters and the gradients must outlive every such graph's last replay.
+ * ntcb_adamw_captured: whether a call with this plan was ever captured. */
 void ntcb_adamw_destroy(ntcb_adamw* a);
+int ntcb_adamw_captured(const ntcb_adamw* a);
 size_t ntcb_adamw_state_bytes(const ntcb_adamw* a);
 long long ntcb_adamw_offset(const ntcb_adamw* a, int tensor);   /* tensor == ntensors: total; -1 out of range */
 /* One step. params[i] / grads[i]: HOST arrays of device pointers; a NULL gradient leaves its tensor and moments as they are. */

@@ -208,6 +208,7 @@ SIGNATURES = {
                                             _vp, C.c_char_p, C.c_size_t]),
     "ntcb_adamw_create": (_vp, [C.c_int, C.c_int, C.POINTER(C.c_longlong), _ip, _ip, C.c_int, C.c_char_p, C.c_size_t]),
     "ntcb_adamw_destroy": (None, [_vp]),
+    "ntcb_adamw_captured": (C.c_int, [_vp]),
     "ntcb_adamw_state_bytes": (C.c_size_t, [_vp]),
     "ntcb_adamw_offset": (C.c_longlong, [_vp, C.c_int]),
     "ntcb_adamw_step": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, C.c_char_p, C.c_size_t]),

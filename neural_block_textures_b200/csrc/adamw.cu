@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cmath>
 #include <new>
@@ -429,6 +430,7 @@ struct ntcb_adamw {
     std::vector<int> param_type, grad_type;
     std::vector<int> first_chunk;              // per tensor, one entry more
     ntcb::Chunk* chunks = nullptr;             // device
+    mutable std::atomic<bool> captured{false}; // a graph has the table's or the state's address
 };
 
 namespace ntcb {
@@ -460,6 +462,15 @@ struct RelaxedCapture {
     RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
     ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
 };
+
+// Whether the stream is being captured (noted in the plan); -1: it cannot be asked.
+int capturing(const ntcb_adamw* a, cudaStream_t s) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(s, &cap) != cudaSuccess) { cudaGetLastError(); return -1; }
+    if (cap == cudaStreamCaptureStatusNone) return 0;
+    a->captured.store(true);
+    return 1;
+}
 
 constexpr int kMaxPerLaunch = 1984;   // two addresses each: 31 KB of the 32 KB that a launch's arguments may take
 
@@ -533,6 +544,8 @@ void ntcb_adamw_destroy(ntcb_adamw* a) {
     delete a;
 }
 
+int ntcb_adamw_captured(const ntcb_adamw* a) { return a && a->captured.load(); }
+
 size_t ntcb_adamw_state_bytes(const ntcb_adamw* a) {
     if (!a) return 0;
     const size_t total = (size_t)a->offset.back();
@@ -565,11 +578,9 @@ int ntcb_adamw_step(const ntcb_adamw* a, void* const* params, const void* const*
     DeviceScope scope(a->device, why, why_cap);
     if (!scope.ok) return 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (!args->it_dev) {   // a replayed step would repeat this step's number
-        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(s, &cap) != cudaSuccess) { cudaGetLastError(); return refuse("the stream cannot be used"); }
-        if (cap != cudaStreamCaptureStatusNone) return refuse("a captured step must take its number from the device (it_dev)");
-    }
+    const int cap = capturing(a, s);
+    if (cap < 0) return refuse("the stream cannot be used");
+    if (cap && !args->it_dev) return refuse("a captured step must take its number from the device (it_dev)");   // a replay would repeat it
     Scalars c{};
     c.lr = args->lr; c.beta1 = args->beta1; c.beta2 = args->beta2; c.wd = args->weight_decay;
     c.log_beta1 = std::log(args->beta1); c.log_beta2 = std::log(args->beta2);
@@ -604,6 +615,7 @@ int ntcb_adamw_get_moments(const ntcb_adamw* a, const void* state, float* m, flo
     DeviceScope scope(a->device, why, why_cap);
     if (!scope.ok) return 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (capturing(a, s) < 0) { set_why(why, why_cap, "the stream cannot be used"); return 0; }
     if (a->bits == 32) {
         cudaError_t e = cudaMemcpyAsync(m, state, (size_t)total * 4, cudaMemcpyDeviceToDevice, s);
         if (e == cudaSuccess) e = cudaMemcpyAsync(v, static_cast<const float*>(state) + total, (size_t)total * 4, cudaMemcpyDeviceToDevice, s);
@@ -624,6 +636,7 @@ int ntcb_adamw_set_moments(const ntcb_adamw* a, const float* m, const float* v, 
     DeviceScope scope(a->device, why, why_cap);
     if (!scope.ok) return 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (capturing(a, s) < 0) { set_why(why, why_cap, "the stream cannot be used"); return 0; }
     if (a->bits == 32) {
         cudaError_t e = cudaMemcpyAsync(state, m, (size_t)total * 4, cudaMemcpyDeviceToDevice, s);
         if (e == cudaSuccess) e = cudaMemcpyAsync(static_cast<float*>(state) + total, v, (size_t)total * 4, cudaMemcpyDeviceToDevice, s);

@@ -9,7 +9,8 @@ the Adam that runs inside the trainer's own steps. With weight_decay 0 it is tha
 
 A step runs on torch's current stream of the parameters' device, without synchronising, and writes the parameters in
 place (autograd does not see that write). In a captured CUDA graph the step number comes from the device: pass `it` as an
-int64 tensor and advance it there.
+int64 tensor and advance it there. The graph has the addresses of the parameters, the gradients and the state: keep those
+tensors as long as it is replayed (the state stays by itself until close()).
 """
 from __future__ import annotations
 
@@ -23,6 +24,7 @@ from . import abi
 from .symbols import DTYPES, _call, _host, _raw_stream
 
 _T = torch.Tensor
+_outlived = []   # (plan, state) of collected optimisers that a graph may still step
 _pack_args = struct.Struct("6dqQ3Q").pack   # ntcb_adamw_args
 
 
@@ -78,12 +80,17 @@ class AdamW:
             self._mv = self.state.view(torch.float32).split(self.offsets[-1]) if self.offsets[-1] else (self.state.view(torch.float32),) * 2
 
     def close(self) -> None:
+        """Frees the plan. No graph that captured a call may be replayed after this; an optimiser that is merely collected
+        leaves the plan and the state of captured calls in place."""
         if getattr(self, "h", None):
             self.lib.ntcb_adamw_destroy(self.h)
             self.h = None
 
     def __del__(self) -> None:
         try:
+            if getattr(self, "h", None) and self.lib.ntcb_adamw_captured(self.h):
+                _outlived.append((self.h, self.state))
+                self.h = None
             self.close()
         except Exception:
             pass

@@ -400,3 +400,38 @@ def test_first_step_on_another_stream_at_once(bits, cuda_device):
                 opt.step(1, 0.25, [g])
                 assert ((p - 0.75).abs() < 1e-5).all()
             torch.cuda.current_stream().wait_stream(stream)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_graph_outlives_the_optimiser(bits, cuda_device):
+    """A captured step goes on working after the object that made it was collected: its plan and its state stay."""
+    import gc
+    import weakref
+    sizes = [70001, 300, 5]
+    a, b, g = tensors(sizes, "f32", 1, 0.5), tensors(sizes, "f32", 1, 0.5), tensors(sizes, "f32", 2, 0.1)
+    it, lr = torch.zeros(1, dtype=torch.int64, device="cuda"), torch.tensor([0.01], device="cuda")
+    opt = AdamW(a, state_bits=bits, seed=3)
+    never = AdamW(a[1:2], state_bits=bits)
+    assert not opt.lib.ntcb_adamw_captured(opt.h)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        it.add_(1)
+        opt.step(it, lr, g)
+        m, v = opt.moments_flat()
+    assert opt.lib.ntcb_adamw_captured(opt.h) and not never.lib.ntcb_adamw_captured(never.h)
+    gone = weakref.ref(opt)
+    del opt, never
+    gc.collect()
+    assert gone() is None
+    torch.cuda.empty_cache()
+    other = [torch.full((1 << k,), 7, dtype=torch.uint8, device="cuda") for k in range(8, 22)]   # takes what was given back
+    eager = AdamW(b, state_bits=bits, seed=3)
+    for k in (1, 2, 3):
+        graph.replay()
+        eager.step(k, float(np.float32(0.01)), g)
+    torch.cuda.synchronize()
+    for x, y in zip(a, b):
+        assert ((x - y).abs() <= 3 * (2 * U * y.abs() + 4 * U * 0.1)).all()
+    assert all(torch.equal(x, y) for x, y in zip((m, v), eager.moments_flat()))
+    assert all((o == 7).all() for o in other)
