@@ -2,9 +2,12 @@
 // tensor or argument costs 40 ns to 2 us, which is 15 us for one small rating and 130 us for an AdamW step over 300
 // tensors. These functions look at the same things and make the same calls of the C ABI (include/ntc_b200.h). Anything
 // but the plain case is left to the Python code, which names what is wrong: they return None (or an index) then.
-// Called through ctypes.PyDLL, so with the interpreter's lock held; a Python exception that is set is raised there.
+// Called through ctypes.PyDLL, so with the interpreter's lock held; a Python exception that is set is raised there. A C++
+// exception must not leave an entry (it would end the process): torch throws them from as little as a size() of a tensor
+// subclass or a nested tensor, so everything is done inside torch's own translation to Python's exceptions.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
@@ -21,7 +24,9 @@ int symbol_code(at::ScalarType t) {
 }
 // A tensor whose memory holds its values as they are: a negated view (the imaginary part of a conjugate) holds their negatives.
 bool plain(PyObject* o) {
-    return THPVariable_Check(o) && THPVariable_Unpack(o).layout() == at::kStrided && !THPVariable_Unpack(o).is_neg();
+    if (!THPVariable_Check(o)) return false;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    return t.layout() == at::kStrided && !t.is_nested() && !t.is_neg();
 }
 
 // The description of plain logits [n, V] and symbols [n] on one CUDA device; false for anything else.
@@ -52,9 +57,9 @@ extern "C" {
 
 // (logp, entropy, lse, top_ids, top_logp), or None.
 PyObject* ntcb_host_logprobs(PyObject* logits, PyObject* symbols, int topk) {
-    ntcb_symbol_desc d;
-    if (!describe(logits, symbols, d) || topk < 0 || topk > NTCB_MAX_TOPK || topk > d.vocab) Py_RETURN_NONE;
-    try {
+    HANDLE_TH_ERRORS
+        ntcb_symbol_desc d;
+        if (!describe(logits, symbols, d) || topk < 0 || topk > NTCB_MAX_TOPK || topk > d.vocab) Py_RETURN_NONE;
         const at::Tensor &x = THPVariable_Unpack(logits), &s = THPVariable_Unpack(symbols);
         const auto f = at::TensorOptions().dtype(at::kFloat).device(x.device());
         const at::Tensor out[5] = {at::empty({d.rows}, f), at::empty({d.rows}, f), at::empty({d.rows}, f),
@@ -71,17 +76,17 @@ PyObject* ntcb_host_logprobs(PyObject* logits, PyObject* symbols, int topk) {
             PyTuple_SET_ITEM(r, i, t);
         }
         return r;
-    } catch (const std::exception& e) { return failed("symbol_logprobs", e.what()); }
+    END_HANDLE_TH_ERRORS
 }
 
 // The gradient in a new tensor, or None. entropy and dentropy may be None.
 PyObject* ntcb_host_logprobs_grad(PyObject* logits, PyObject* symbols, PyObject* lse, PyObject* entropy, PyObject* dlogp, PyObject* dentropy) {
-    ntcb_symbol_desc d;
-    if (!describe(logits, symbols, d) || !per_row(lse, d) || !per_row(dlogp, d)) Py_RETURN_NONE;
-    const bool with = dentropy != Py_None;
-    if (with && (!per_row(dentropy, d) || !per_row(entropy, d) || !THPVariable_Unpack(entropy).is_contiguous())) Py_RETURN_NONE;
-    if (!THPVariable_Unpack(lse).is_contiguous()) Py_RETURN_NONE;
-    try {
+    HANDLE_TH_ERRORS
+        ntcb_symbol_desc d;
+        if (!describe(logits, symbols, d) || !per_row(lse, d) || !per_row(dlogp, d)) Py_RETURN_NONE;
+        const bool with = dentropy != Py_None;
+        if (with && (!per_row(dentropy, d) || !per_row(entropy, d) || !THPVariable_Unpack(entropy).is_contiguous())) Py_RETURN_NONE;
+        if (!THPVariable_Unpack(lse).is_contiguous()) Py_RETURN_NONE;
         const at::Tensor &x = THPVariable_Unpack(logits), &l = THPVariable_Unpack(dlogp);
         const at::Tensor out = at::empty({d.rows, d.vocab}, at::TensorOptions().dtype(x.scalar_type()).device(x.device()));
         char why[256];
@@ -91,11 +96,12 @@ PyObject* ntcb_host_logprobs_grad(PyObject* logits, PyObject* symbols, PyObject*
                                        with ? THPVariable_Unpack(dentropy).stride(0) : 0, out.data_ptr(), d.vocab, stream_of(d.device), why, sizeof(why)))
             return failed("symbol_logprobs_grad", why);
         return THPVariable_Wrap(out);
-    } catch (const std::exception& e) { return failed("symbol_logprobs_grad", e.what()); }
+    END_HANDLE_TH_ERRORS
 }
 
 // The addresses of n parameters and gradients (lists; a gradient may be None: 0 for both) after checking sizes, types,
-// layout and device. Returns -1, or the index of the first tensor that does not fit, or -2 when the lists do not.
+// layout and device. Returns -1, or the index of the first tensor that does not fit (with the Python exception that it
+// raised, if it did), or -2 when the lists do not.
 int ntcb_host_addresses(PyObject* params, PyObject* grads, int n, const long long* sizes, const int* param_types, const int* grad_types,
                         int device, uint64_t* pp, uint64_t* gg) {
     if (!PyList_Check(params) || !PyList_Check(grads) || PyList_GET_SIZE(params) != n || PyList_GET_SIZE(grads) != n) return -2;
@@ -104,8 +110,9 @@ int ntcb_host_addresses(PyObject* params, PyObject* grads, int n, const long lon
         const at::Tensor& t = THPVariable_Unpack(o);
         return t.numel() == size && dtype_code(t.scalar_type()) == type && t.is_contiguous() && t.is_cuda() && t.get_device() == device;
     };
+    int i = 0;
     try {
-        for (int i = 0; i < n; i++) {
+        for (; i < n; i++) {
             PyObject *p = PyList_GET_ITEM(params, i), *g = PyList_GET_ITEM(grads, i);
             pp[i] = gg[i] = 0;
             if (g == Py_None) continue;
@@ -113,8 +120,11 @@ int ntcb_host_addresses(PyObject* params, PyObject* grads, int n, const long lon
             pp[i] = reinterpret_cast<uint64_t>(THPVariable_Unpack(p).data_ptr());
             gg[i] = reinterpret_cast<uint64_t>(THPVariable_Unpack(g).data_ptr());
         }
-    } catch (const std::exception&) { return -2; }
-    return -1;
+    } catch (python_error& e) {
+        e.restore();
+    } catch (...) {   // a tensor that does not say what it is, or has no memory
+    }
+    return i < n ? i : -1;
 }
 
 }  // extern "C"

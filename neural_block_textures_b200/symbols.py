@@ -39,6 +39,8 @@ def _desc(logits: torch.Tensor, symbols: torch.Tensor, name: str) -> tuple[bytes
     """(ntcb_symbol_desc, rows, vocab, device index) of checked arguments."""
     if not isinstance(logits, torch.Tensor) or not isinstance(symbols, torch.Tensor):
         raise TypeError(f"{name}: logits and symbols must be torch tensors")
+    if any(x.layout is not torch.strided or x.is_nested for x in (logits, symbols)):
+        raise ValueError(f"{name}: logits and symbols must be strided tensors, not sparse or nested ones")
     dtype, symbol_type = DTYPES.get(logits.dtype), SYMBOL_TYPES.get(symbols.dtype)
     if dtype is None:
         raise TypeError(f"{name}: logits must be float32, float16 or bfloat16, not {logits.dtype}")
@@ -101,7 +103,7 @@ def symbol_logprobs(logits: torch.Tensor, symbols: torch.Tensor, topk: int = 0) 
         return symbol_logprobs(logits.resolve_neg(), symbols, topk)
     if not 0 <= topk <= min(abi.MAX_TOPK, v):
         raise ValueError(f"symbol_logprobs: topk must be 0 .. {min(abi.MAX_TOPK, v)} here, not {topk}")
-    raise ValueError("symbol_logprobs: logits and symbols must be strided tensors")
+    raise ValueError("symbol_logprobs: these tensors cannot be rated")
 
 
 def symbol_logprobs_grad(logits: torch.Tensor, symbols: torch.Tensor, lse: torch.Tensor, entropy: torch.Tensor | None,

@@ -508,3 +508,18 @@ def test_negated_views(cuda_device):
     assert torch.equal(da, db)
     with pytest.raises(ValueError, match="negated"):
         symbol_logprobs_grad(x[:, :1], z, a.lse, a.entropy, -1.0, out=one)
+
+
+def test_nested_tensors_and_memory_that_runs_out(cuda_device):
+    """torch's own exceptions arrive as what they are."""
+    nested = torch.nested.nested_tensor([torch.zeros(3, device="cuda"), torch.zeros(5, device="cuda")])
+    s = torch.zeros(2, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="nested"):
+        symbol_logprobs(nested, s)
+    with pytest.raises(ValueError, match="nested"):
+        symbol_logprobs_grad(nested, s, s.float(), None, s.float())
+    row, none = torch.zeros(1, 1 << 20, device="cuda"), torch.zeros(1, dtype=torch.uint8, device="cuda")
+    n = 1 << 19   # rows of one shared row: a gradient of 2 TB
+    per_row = torch.zeros(1, device="cuda").expand(n)
+    with pytest.raises(torch.OutOfMemoryError):
+        symbol_logprobs_grad(row.expand(n, 1 << 20), none.expand(n), torch.zeros(n, device="cuda"), None, per_row)

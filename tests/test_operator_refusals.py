@@ -4,6 +4,7 @@ C layout."""
 import ctypes as C
 import shutil
 import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -158,3 +159,51 @@ def test_eps_below_the_normal_numbers_is_refused():
     for eps in (1e-40, 1.17e-38, 5e-324):
         with pytest.raises(ValueError, match="eps"):
             AdamW([torch.zeros(4, 8)], eps=eps)
+
+
+HOSTILE = """
+import ctypes, torch
+from array import array
+from neural_block_textures_b200 import AdamW, symbol_logprobs, symbol_logprobs_grad
+from neural_block_textures_b200.symbols import _host
+
+class Hostile(torch.Tensor):   # says that it is on a CUDA device and raises on every question about its shape
+    @staticmethod
+    def __new__(cls):
+        return torch.Tensor._make_wrapper_subclass(cls, (4, 8), dtype=torch.float32, device="cuda", dispatch_sizes_strides_policy="sizes")
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise KeyError(str(func))
+
+x, s = Hostile(), torch.zeros(4, dtype=torch.int64)
+for call in (lambda: symbol_logprobs(x, s), lambda: symbol_logprobs_grad(x, s, s.float(), None, s.float()), lambda: AdamW([x])):
+    try:
+        call()
+        raise SystemExit("no exception")
+    except KeyError as e:
+        assert "aten" in str(e)
+one = (ctypes.c_longlong * 1)(32), (ctypes.c_int * 1)(0), (ctypes.c_int * 1)(0)
+pp, gg = array("Q", [0]), array("Q", [0])
+try:
+    _host.ntcb_host_addresses([x], [x], 1, *[ctypes.addressof(a) for a in one], 0, pp.buffer_info()[0], gg.buffer_info()[0])
+    raise SystemExit("no exception")
+except KeyError:
+    print("fine")
+"""
+
+
+def test_exceptions_of_tensors_reach_python():
+    """A tensor subclass that raises where its sizes are asked for: its exception arrives, and the process goes on."""
+    r = subprocess.run([sys.executable, "-c", HOSTILE], capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
+
+
+def test_nested_and_sparse_tensors_are_refused():
+    s = torch.zeros(4, dtype=torch.int64)
+    nested = torch.nested.nested_tensor([torch.zeros(3), torch.zeros(5)])
+    jagged = torch.nested.nested_tensor([torch.zeros(3), torch.zeros(5)], layout=torch.jagged)
+    for x in (nested, jagged, torch.zeros(4, 8).to_sparse()):
+        with pytest.raises(ValueError, match="strided"):
+            symbol_logprobs(x, s)
+        with pytest.raises(ValueError, match="strided"):
+            symbol_logprobs_grad(x, s, s.float(), None, -1.0)
