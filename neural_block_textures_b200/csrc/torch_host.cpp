@@ -2,7 +2,7 @@
 // tensor or argument costs 40 ns to 2 us, which is 15 us for one small rating and 130 us for an AdamW step over 300
 // tensors. These functions look at the same things and make the same calls of the C ABI (include/ntc_b200.h). Anything
 // but the plain case is left to the Python code, which names what is wrong: they return None (or an index) then.
-// Called through ctypes.PyDLL, so with the interpreter's lock held; a Python exception that is set is raised there. A C++
+// Called through ctypes.PyDLL, so with the interpreter's lock held (and let go while they allocate and launch); a Python exception that is set is raised there. A C++
 // exception must not leave an entry (it would end the process): torch throws them from as little as a size() of a tensor
 // subclass or a nested tensor, so everything is done inside torch's own translation to Python's exceptions.
 #include <ATen/ATen.h>
@@ -46,6 +46,13 @@ bool per_row(PyObject* o, const ntcb_symbol_desc& d) {
 }
 void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream(); }
 
+// The interpreter's lock let go: an allocation may wait for the device and a launch for a place in its queue, and what is
+// queued there may be a host function that needs the lock.
+struct Unlocked {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 PyObject* failed(const char* name, const char* why) {
     PyErr_Format(PyExc_RuntimeError, "%s: %s", name, why);
     return nullptr;
@@ -60,14 +67,20 @@ PyObject* ntcb_host_logprobs(PyObject* logits, PyObject* symbols, int topk) {
     HANDLE_TH_ERRORS
         ntcb_symbol_desc d;
         if (!describe(logits, symbols, d) || topk < 0 || topk > NTCB_MAX_TOPK || topk > d.vocab) Py_RETURN_NONE;
-        const at::Tensor &x = THPVariable_Unpack(logits), &s = THPVariable_Unpack(symbols);
-        const auto f = at::TensorOptions().dtype(at::kFloat).device(x.device());
-        const at::Tensor out[5] = {at::empty({d.rows}, f), at::empty({d.rows}, f), at::empty({d.rows}, f),
-                                   at::empty({d.rows, topk}, f.dtype(at::kInt)), at::empty({d.rows, topk}, f)};
+        const at::Tensor x = THPVariable_Unpack(logits), s = THPVariable_Unpack(symbols);
+        at::Tensor out[5];
         char why[256];
-        if (!ntcb_symbol_logprobs(&d, x.data_ptr(), s.data_ptr(), topk, out[0].data_ptr<float>(), out[1].data_ptr<float>(),
-                                  out[2].data_ptr<float>(), out[3].data_ptr<int>(), out[4].data_ptr<float>(), stream_of(d.device), why, sizeof(why)))
-            return failed("symbol_logprobs", why);
+        bool ok;
+        {
+            const Unlocked unlocked;
+            const auto f = at::TensorOptions().dtype(at::kFloat).device(x.device());
+            for (int i = 0; i < 3; i++) out[i] = at::empty({d.rows}, f);
+            out[3] = at::empty({d.rows, topk}, f.dtype(at::kInt));
+            out[4] = at::empty({d.rows, topk}, f);
+            ok = ntcb_symbol_logprobs(&d, x.data_ptr(), s.data_ptr(), topk, out[0].data_ptr<float>(), out[1].data_ptr<float>(),
+                                      out[2].data_ptr<float>(), out[3].data_ptr<int>(), out[4].data_ptr<float>(), stream_of(d.device), why, sizeof(why));
+        }
+        if (!ok) return failed("symbol_logprobs", why);
         PyObject* r = PyTuple_New(5);
         if (!r) return nullptr;
         for (int i = 0; i < 5; i++) {
@@ -87,14 +100,19 @@ PyObject* ntcb_host_logprobs_grad(PyObject* logits, PyObject* symbols, PyObject*
         const bool with = dentropy != Py_None;
         if (with && (!per_row(dentropy, d) || !per_row(entropy, d) || !THPVariable_Unpack(entropy).is_contiguous())) Py_RETURN_NONE;
         if (!THPVariable_Unpack(lse).is_contiguous()) Py_RETURN_NONE;
-        const at::Tensor &x = THPVariable_Unpack(logits), &l = THPVariable_Unpack(dlogp);
-        const at::Tensor out = at::empty({d.rows, d.vocab}, at::TensorOptions().dtype(x.scalar_type()).device(x.device()));
+        const at::Tensor x = THPVariable_Unpack(logits), s = THPVariable_Unpack(symbols), sum = THPVariable_Unpack(lse), l = THPVariable_Unpack(dlogp);
+        const at::Tensor h = with ? THPVariable_Unpack(entropy) : at::Tensor(), e = with ? THPVariable_Unpack(dentropy) : at::Tensor();
+        at::Tensor out;
         char why[256];
-        if (!ntcb_symbol_logprobs_grad(&d, x.data_ptr(), THPVariable_Unpack(symbols).data_ptr(), THPVariable_Unpack(lse).data_ptr<float>(),
-                                       with ? THPVariable_Unpack(entropy).data_ptr<float>() : nullptr, l.data_ptr<float>(), l.stride(0),
-                                       with ? THPVariable_Unpack(dentropy).data_ptr<float>() : nullptr,
-                                       with ? THPVariable_Unpack(dentropy).stride(0) : 0, out.data_ptr(), d.vocab, stream_of(d.device), why, sizeof(why)))
-            return failed("symbol_logprobs_grad", why);
+        bool ok;
+        {
+            const Unlocked unlocked;
+            out = at::empty({d.rows, d.vocab}, at::TensorOptions().dtype(x.scalar_type()).device(x.device()));
+            ok = ntcb_symbol_logprobs_grad(&d, x.data_ptr(), s.data_ptr(), sum.data_ptr<float>(), with ? h.data_ptr<float>() : nullptr,
+                                           l.data_ptr<float>(), l.stride(0), with ? e.data_ptr<float>() : nullptr, with ? e.stride(0) : 0,
+                                           out.data_ptr(), d.vocab, stream_of(d.device), why, sizeof(why));
+        }
+        if (!ok) return failed("symbol_logprobs_grad", why);
         return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }

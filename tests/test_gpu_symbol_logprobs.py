@@ -523,3 +523,35 @@ def test_nested_tensors_and_memory_that_runs_out(cuda_device):
     per_row = torch.zeros(1, device="cuda").expand(n)
     with pytest.raises(torch.OutOfMemoryError):
         symbol_logprobs_grad(row.expand(n, 1 << 20), none.expand(n), torch.zeros(n, device="cuda"), None, per_row)
+
+
+def test_other_threads_run_while_a_call_waits_for_the_queue(cuda_device):
+    """More calls than the launch queue holds behind about half a second of device work: a call that waits for a place in
+    it does not hold the interpreter."""
+    import threading
+    import time
+    x, s, _, _ = make(6, 9, "f32", masks=False)
+    one, half = torch.full((6,), -1.0, device="cuda"), torch.full((6,), 0.5, device="cuda")
+    r = symbol_logprobs(x, s)
+    symbol_logprobs_grad(x, s, r.lse, r.entropy, one, half)
+    torch.cuda.synchronize()
+    for call in (lambda: symbol_logprobs(x, s), lambda: symbol_logprobs_grad(x, s, r.lse, r.entropy, one, half)):
+        longest, done = [0.0], threading.Event()
+
+        def tick():
+            last = time.perf_counter()
+            while not done.is_set():
+                time.sleep(0.0005)
+                now = time.perf_counter()
+                longest[0], last = max(longest[0], now - last), now
+        thread = threading.Thread(target=tick)
+        thread.start()
+        torch.cuda._sleep(1_000_000_000)   # device clocks
+        begin = time.perf_counter()
+        for _ in range(3000):
+            call()
+        took = time.perf_counter() - begin
+        done.set()
+        thread.join()
+        torch.cuda.synchronize()
+        assert longest[0] < max(0.1, took / 4), (longest, took)
