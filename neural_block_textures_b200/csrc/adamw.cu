@@ -569,6 +569,8 @@ int ntcb_adamw_step(const ntcb_adamw* a, void* const* params, const void* const*
     if (args->eps > 0.0 && args->eps < (double)FLT_MIN) return refuse("eps must be 0 or a normal 32-bit number (1.18e-38 or more)");
     if (!args->lr_dev && !(std::isfinite(args->lr) && args->lr >= 0.0)) return refuse("lr must be finite and not negative");
     if (!args->it_dev && (args->it < 1 || args->it > 0xffffffffll)) return refuse("it counts from 1 and stays below 2^32");
+    if (reinterpret_cast<uintptr_t>(args->it_dev) % 8 || reinterpret_cast<uintptr_t>(args->lr_dev) % 4 || reinterpret_cast<uintptr_t>(args->grad_scale_dev) % 4)
+        return refuse("a device scalar is not aligned to its type");
     for (int i = 0; i < n; i++) {
         if (!a->size[(size_t)i] || !grads[i]) continue;
         if (!params[i]) return refuse("null parameter");

@@ -48,7 +48,9 @@ extern "C" int ntcb_symbol_logprobs(const ntcb_symbol_desc* d, const void* logit
     if (topk > d->vocab) return refuse("topk above vocab");
     if (d->rows == 0) return 1;
     if (!logits || !symbols || !logp || !entropy || !lse || (topk && (!top_ids || !top_logp))) return refuse("null buffer");
-    if (!aligned(logits, dtype_size(d->dtype)) || !aligned(symbols, symbol_size(d->symbol_type))) return refuse("a buffer is not aligned to its type");
+    if (!aligned(logits, dtype_size(d->dtype)) || !aligned(symbols, symbol_size(d->symbol_type)) || !aligned(logp, 4) || !aligned(entropy, 4) ||
+        !aligned(lse, 4) || (topk && (!aligned(top_ids, 4) || !aligned(top_logp, 4))))
+        return refuse("a buffer is not aligned to its type");
     DeviceScope scope(d->device, why, why_cap);
     if (!scope.ok) return 0;
     const RowArgs a{logits, symbols, d->rows, d->row_stride, d->symbol_stride, (int)d->vocab, topk, d->symbol_type,
@@ -72,7 +74,9 @@ extern "C" int ntcb_symbol_logprobs_grad(const ntcb_symbol_desc* d, const void* 
     if (d->rows == 0) return 1;
     if (!logits || !symbols || !lse || !dlogp || !dlogits || (dentropy && !entropy)) return refuse("null buffer");
     const size_t sz = dtype_size(d->dtype);
-    if (!aligned(logits, sz) || !aligned(dlogits, sz) || !aligned(symbols, symbol_size(d->symbol_type))) return refuse("a buffer is not aligned to its type");
+    if (!aligned(logits, sz) || !aligned(dlogits, sz) || !aligned(symbols, symbol_size(d->symbol_type)) || !aligned(lse, 4) || !aligned(dlogp, 4) ||
+        (dentropy && (!aligned(dentropy, 4) || !aligned(entropy, 4))))
+        return refuse("a buffer is not aligned to its type");
     if (!may_write(logits, d->row_stride, dlogits, dlogits_stride, d->rows, d->vocab, sz)) return refuse("dlogits overlaps the logits without being them");
     DeviceScope scope(d->device, why, why_cap);
     if (!scope.ok) return 0;

@@ -435,3 +435,21 @@ def test_a_graph_outlives_the_optimiser(bits, cuda_device):
         assert ((x - y).abs() <= 3 * (2 * U * y.abs() + 4 * U * 0.1)).all()
     assert all(torch.equal(x, y) for x, y in zip((m, v), eager.moments_flat()))
     assert all((o == 7).all() for o in other)
+
+
+def test_device_scalars_off_their_alignment(cuda_device):
+    """Refused by the C entry before anything is launched."""
+    import ctypes as C
+
+    from neural_block_textures_b200 import abi
+    p, g = torch.ones(8, device="cuda"), torch.ones(8, device="cuda")
+    opt = AdamW([p])
+    spare = torch.zeros(4, dtype=torch.int64, device="cuda").data_ptr()
+    why = C.create_string_buffer(256)
+    for name, off in (("it_dev", 4), ("lr_dev", 2), ("grad_scale_dev", 1)):
+        args = abi.AdamWArgs(lr=0.1, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, grad_scale=1.0, it=1, seed=0)
+        setattr(args, name, spare + off)
+        ok = opt.lib.ntcb_adamw_step(opt.h, (C.c_void_p * 1)(p.data_ptr()), (C.c_void_p * 1)(g.data_ptr()), opt.state.data_ptr(),
+                                     C.addressof(args), None, why, 256)
+        assert ok == 0 and b"aligned" in why.value
+    assert (p == 1).all()

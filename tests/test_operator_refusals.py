@@ -207,3 +207,15 @@ def test_nested_and_sparse_tensors_are_refused():
             symbol_logprobs(x, s)
         with pytest.raises(ValueError, match="strided"):
             symbol_logprobs_grad(x, s, s.float(), None, -1.0)
+
+
+def test_buffers_off_their_alignment():
+    """Every buffer, not the logits and symbols alone: a 32-bit access off its boundary would fault the device."""
+    lib, why = abi.load_library(), C.create_string_buffer(256)
+    d = C.byref(desc())
+    for bad in range(5):
+        out = [BUF + 2 * (i == bad) for i in range(5)]
+        assert lib.ntcb_symbol_logprobs(d, BUF, BUF, 2, *out, None, why, 256) == 0 and b"aligned" in why.value
+    for bad in range(4):   # lse, entropy, dlogp, dentropy
+        lse, entropy, dlogp, dentropy = [BUF + 2 * (i == bad) for i in range(4)]
+        assert lib.ntcb_symbol_logprobs_grad(d, BUF, BUF, lse, entropy, dlogp, 1, dentropy, 1, BUF, 8, None, why, 256) == 0 and b"aligned" in why.value
