@@ -392,7 +392,8 @@ int ntcb_symbol_logprobs(const ntcb_symbol_desc* d, const void* logits, const vo
  * are the forward pass's (entropy is read only with dentropy, which may be NULL). The strides of dlogp and dentropy
  * may be 0 (one value for every row). dlogits may be the logits' own buffer with their stride. Rows without a finite
  * logit and, for the logp part, rows without a symbol get 0; rows the forward pass gave NaN get NaN. Rows whose lse is 256
- * or more in size (its rounding then shows in the probabilities) are normalised anew from the logits. */
+ * or more in size (its rounding then shows in the probabilities) are normalised anew from the logits: such a row is read
+ * two to nine times. */
 int ntcb_symbol_logprobs_grad(const ntcb_symbol_desc* d, const void* logits, const void* symbols, const float* lse, const float* entropy,
                               const float* dlogp, long long dlogp_stride, const float* dentropy, long long dentropy_stride, void* dlogits,
                               long long dlogits_stride, void* stream, char* why, size_t why_cap);

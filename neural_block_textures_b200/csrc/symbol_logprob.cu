@@ -81,10 +81,10 @@ extern "C" int ntcb_symbol_logprobs_grad(const ntcb_symbol_desc* d, const void* 
     DeviceScope scope(d->device, why, why_cap);
     if (!scope.ok) return 0;
     const GradArgs a{logits, symbols, lse, entropy, dlogp, dentropy, dlogits, d->rows, d->row_stride, d->symbol_stride, dlogits_stride,
-                     dlogp_stride, dentropy_stride, (int)d->vocab, d->symbol_type, 0};
+                     dlogp_stride, dentropy_stride, (int)d->vocab, d->symbol_type, 1, 1};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = d->dtype == NTCB_F32 ? symbol_grad_f32(a, s)
-                          : d->dtype == NTCB_F16 ? symbol_grad_f16(a, s)
-                                                 : symbol_grad_bf16(a, s);
+    const cudaError_t e = d->dtype == NTCB_F32 ? symbol_grad_f32(a, s, scope.sms)
+                          : d->dtype == NTCB_F16 ? symbol_grad_f16(a, s, scope.sms)
+                                                 : symbol_grad_bf16(a, s, scope.sms);
     return scope.launched(e, why, why_cap);
 }

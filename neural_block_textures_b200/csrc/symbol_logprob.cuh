@@ -785,15 +785,24 @@ __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, i
 
 // -------------------------------------------------------------------------------------------------------- gradient
 
-// The sum of a row's exponentials relative to its lse, by the row's `group` threads (at most a warp's, or a CTA).
+// The sum of a row's exponentials relative to its lse, by the row's `group` threads (at most a warp's, or a CTA), which take
+// four vectors at a time.
 template <class T, bool CTA>
 __device__ __forceinline__ float row_sum(const T* row, int V, int shift, int lane, int group, float lse) {
-    constexpr int N = VEC<T>;
+    constexpr int N = VEC<T>, U = CTA ? 4 : 1;
     const Scale sc(lse);
     float2 s2 = make_float2(0.0f, 0.0f), u2 = s2;
-    for (int c = lane; c * N - shift < V; c += group) {
-        const uint4 one[1] = {load_vec<false>(row, c * N - shift, V)};
-        add_exp<T>(one, sc, s2, u2);
+    for (int c = lane; c * N - shift < V; c += U * group) {
+        uint4 raw[U];
+#pragma unroll
+        for (int k = 0; k < U; k++) raw[k] = load_vec<false>(row, (c + k * group) * N - shift, V);
+        if constexpr (CTA) {   // a round's sum by itself: rows may be long
+            float2 e2 = make_float2(0.0f, 0.0f);
+            add_exp<T>(raw, sc, e2, u2);
+            s2 = __fadd2_rn(s2, e2);
+        } else {
+            add_exp<T>(raw, sc, s2, u2);
+        }
     }
     float s = s2.x + s2.y;
     if constexpr (CTA) {
@@ -832,7 +841,9 @@ __global__ void __launch_bounds__(256, M == 1 ? 8 : 5) k_logprobs_grad(const Gra
     const T* row = static_cast<const T*>(a.x) + r * a.stride;
     T* out = static_cast<T*>(a.dx) + r * a.dx_stride;
     const int shift = row_shift(row), V = a.V, nvec = (V + shift + N - 1) / N;
-    int c0 = lane + (CTA ? (int)(blockIdx.x % (unsigned)a.chunks) * M * group : 0);
+    const int part = CTA ? (int)(blockIdx.x % (unsigned)a.chunks) : 0;
+    int parts = CTA ? a.chunks : 1;   // CTAs that share the row
+    int c0 = lane + part * M * group;
     uint4 raw[M];
 #pragma unroll
     for (int k = 0; k < M; k++) raw[k] = load_vec<false>(row, (c0 + k * group) * N - shift, V);
@@ -845,9 +856,17 @@ __global__ void __launch_bounds__(256, M == 1 ? 8 : 5) k_logprobs_grad(const Gra
     float p0 = -fmaf(sc.off, kLn2, 1.0f);   // p = -p0 2^y (2^off, or 1 / sum)
     float shift_nat = sc.off * kLn2;        // log p = y ln 2 + shift_nat
     if (!empty && fabsf(lse) >= 256.0f) {
+        if constexpr (CTA) {
+            parts = min(parts, a.far_parts);
+            if (part >= parts) return;   // the whole CTA
+        }
         const float s = row_sum<T, CTA>(row, V, shift, lane, group, lse);
         p0 = __fdividef(-1.0f, s);
         shift_nat = -logf(s);
+        if constexpr (CTA) {   // again, rather than kept over the sum
+#pragma unroll
+            for (int k = 0; k < M; k++) raw[k] = load_vec<false>(row, (c0 + k * group) * N - shift, V);
+        }
     }
     float dh = 0.0f, base = dl;
     if constexpr (ENTROPY) {
@@ -906,8 +925,7 @@ __global__ void __launch_bounds__(256, M == 1 ? 8 : 5) k_logprobs_grad(const Gra
             }
         }
         if constexpr (!CTA) return;
-        if (a.chunks > 1) return;
-        c0 += M * group;   // a CTA with a whole row goes on
+        c0 += parts * M * group;   // a CTA with more than one part of the row goes on
         if (c0 - lane >= nvec) return;
 #pragma unroll
         for (int k = 0; k < M; k++) raw[k] = load_vec<false>(row, (c0 + k * group) * N - shift, V);
@@ -1017,7 +1035,7 @@ cudaError_t launch_rows(const RowArgs& a, cudaStream_t s, int sms) {
 }
 
 template <class T, bool ENTROPY>
-cudaError_t launch_grad(GradArgs a, cudaStream_t s) {
+cudaError_t launch_grad(GradArgs a, cudaStream_t s, int sms) {
     const int nvec = (int)ceil_div(row_span<T>(a.x, a.stride, a.V), VEC<T>);
     int lg = 0;
     a.chunks = 1;
@@ -1031,12 +1049,15 @@ cudaError_t launch_grad(GradArgs a, cudaStream_t s) {
     } else {
         const int threads = nvec <= 256 ? 64 : nvec <= 512 ? 128 : 256;
         if (a.dx != a.x) a.chunks = (int)ceil_div(nvec, 4 * threads);
+        a.far_parts = (int)std::min<long long>(8, std::max<long long>(1, 4 * sms / a.rows));   // few rows: more of each at once
         k_logprobs_grad<T, 4, ENTROPY, true><<<(unsigned)(a.rows * a.chunks), threads, 0, s>>>(a, 0);
     }
     return cudaGetLastError();
 }
 template <class T>
-cudaError_t launch_grad(const GradArgs& a, cudaStream_t s) { return a.dentropy ? launch_grad<T, true>(a, s) : launch_grad<T, false>(a, s); }
+cudaError_t launch_grad(const GradArgs& a, cudaStream_t s, int sms) {
+    return a.dentropy ? launch_grad<T, true>(a, s, sms) : launch_grad<T, false>(a, s, sms);
+}
 
 }  // namespace
 }  // namespace ntcb

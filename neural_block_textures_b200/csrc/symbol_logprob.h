@@ -20,14 +20,14 @@ struct GradArgs {
     const float *lse, *entropy, *dlogp, *dentropy;
     void* dx;
     long long rows, stride, sym_stride, dx_stride, dlogp_stride, dentropy_stride;
-    int V, sym_type, chunks;
+    int V, sym_type, chunks, far_parts;
 };
 
 cudaError_t symbol_rows_f32(const RowArgs& a, cudaStream_t s, int sms);
 cudaError_t symbol_rows_f16(const RowArgs& a, cudaStream_t s, int sms);
 cudaError_t symbol_rows_bf16(const RowArgs& a, cudaStream_t s, int sms);
-cudaError_t symbol_grad_f32(const GradArgs& a, cudaStream_t s);
-cudaError_t symbol_grad_f16(const GradArgs& a, cudaStream_t s);
-cudaError_t symbol_grad_bf16(const GradArgs& a, cudaStream_t s);
+cudaError_t symbol_grad_f32(const GradArgs& a, cudaStream_t s, int sms);
+cudaError_t symbol_grad_f16(const GradArgs& a, cudaStream_t s, int sms);
+cudaError_t symbol_grad_bf16(const GradArgs& a, cudaStream_t s, int sms);
 
 }  // namespace ntcb

@@ -3,5 +3,5 @@
 
 namespace ntcb {
 cudaError_t symbol_rows_f16(const RowArgs& a, cudaStream_t s, int sms) { return launch_rows<__half>(a, s, sms); }
-cudaError_t symbol_grad_f16(const GradArgs& a, cudaStream_t s) { return launch_grad<__half>(a, s); }
+cudaError_t symbol_grad_f16(const GradArgs& a, cudaStream_t s, int sms) { return launch_grad<__half>(a, s, sms); }
 }  // namespace ntcb

@@ -3,5 +3,5 @@
 
 namespace ntcb {
 cudaError_t symbol_rows_f32(const RowArgs& a, cudaStream_t s, int sms) { return launch_rows<float>(a, s, sms); }
-cudaError_t symbol_grad_f32(const GradArgs& a, cudaStream_t s) { return launch_grad<float>(a, s); }
+cudaError_t symbol_grad_f32(const GradArgs& a, cudaStream_t s, int sms) { return launch_grad<float>(a, s, sms); }
 }  // namespace ntcb

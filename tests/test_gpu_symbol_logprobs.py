@@ -555,3 +555,46 @@ def test_other_threads_run_while_a_call_waits_for_the_queue(cuda_device):
         thread.join()
         torch.cuda.synchronize()
         assert longest[0] < max(0.1, took / 4), (longest, took)
+
+
+@pytest.mark.parametrize("dtype, n, v", [("f32", 1, 300007), ("f32", 3, 40000), ("bf16", 2, 200001), ("f32", 700, 20000), ("f16", 300, 50001), ("f32", 160, 9001)])
+def test_gradient_of_long_rows_far_from_zero(dtype, n, v, cuda_device):
+    """Rows of many CTAs whose sum is taken anew, few and many of them, beside ordinary ones: the numbers of a call over
+    the logits, and, for the first rows, the formula's."""
+    gen = torch.Generator().manual_seed(v)
+    x = torch.randn(n, v, generator=gen) * 2
+    x[::3] += 1000.0
+    x[1::3] = max(-1e9, torch.finfo(DT[dtype]).min)
+    x[1::3, v // 3] = 2.0
+    if n > 4:
+        x[4] = torch.finfo(DT[dtype]).min
+    x = x.to(DT[dtype])
+    s = torch.randint(0, v, (n,), generator=gen)
+    dl, dh = torch.randn(n, generator=gen).cuda(), torch.randn(n, generator=gen).cuda()
+    few = min(n, 6)
+    check_grad(x[:few].cuda(), s[:few].cuda(), x[:few].double().numpy(), s[:few].numpy(), dl[:few], dh[:few], dtype)
+    x, s = x.cuda(), s.cuda()
+    r = symbol_logprobs(x, s)
+    got = symbol_logprobs_grad(x, s, r.lse, r.entropy, dl, dh)
+    assert torch.equal(symbol_logprobs_grad(x, s, r.lse, r.entropy, dl, dh, out=x), got)
+
+
+def test_cost_of_rows_far_from_zero(cuda_device):
+    """Few CTAs of a long row take its sum anew, so the cost keeps to the row's length: eight times the logits take less
+    than 24 times as long (eight by the bytes; each of a row's CTAs summing all of it would be 64)."""
+    times = []
+    for v in (1 << 20, 1 << 23):
+        x = torch.full((1, v), -1e9, device="cuda")
+        s = torch.zeros(1, dtype=torch.int32, device="cuda")
+        r = symbol_logprobs(x, s)
+        one = torch.ones(1, device="cuda")
+        best = math.inf
+        for _ in range(5):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            symbol_logprobs_grad(x, s, r.lse, r.entropy, one)
+            end.record()
+            end.synchronize()
+            best = min(best, begin.elapsed_time(end))
+        times.append(best)
+    assert times[1] < 24 * times[0], times
