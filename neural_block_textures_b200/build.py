@@ -1,6 +1,6 @@
 """Builds libntc_b200.so (the CUDA kernels, the host engine, the C ABI and the ntc_cuda::Trainer
-class) in-tree with nvcc for sm_100a, and libntc_b200_torch.so (the host side of the operators on torch tensors) with
-the C++ compiler. Run `python -m neural_block_textures_b200.build`."""
+class) in-tree with nvcc for sm_100a, and, where torch is installed, libntc_b200_torch.so (the host side of the operators on
+torch tensors) with the C++ compiler. Run `python -m neural_block_textures_b200.build`."""
 from __future__ import annotations
 
 import concurrent.futures as cf
@@ -62,6 +62,15 @@ def _compile(src: str, verbose: bool) -> Path:
     return obj
 
 
+def _torch_host_lacks() -> str | None:
+    """What keeps the torch library from being built here, if something does. The rest of the package needs neither."""
+    if importlib.util.find_spec("torch") is None:
+        return "torch is not installed"
+    if not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
+        return "Python's headers are not installed"
+    return None
+
+
 def _compile_torch_host() -> Path:
     """torch_host.cpp against the installed torch's headers."""
     s = CSRC / TORCH_SOURCE
@@ -92,16 +101,19 @@ def _link_torch_host(obj: Path) -> None:
 def build(verbose: bool = False) -> Path:
     OUT_DIR.mkdir(exist_ok=True)
     BUILD_DIR.mkdir(exist_ok=True)
+    lacks = _torch_host_lacks()
     with cf.ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
-        host = ex.submit(_compile_torch_host)
+        host = None if lacks else ex.submit(_compile_torch_host)
         objs = list(ex.map(lambda s: _compile(s, verbose), SOURCES))
-        host_obj = host.result()
     if _stale(LIB, objs):
         cmd = [nvcc(), *GENCODE, "-shared", "-Xcompiler", "-fPIC", "-o", str(LIB), *map(str, objs), "-cudart", "static"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
-    _link_torch_host(host_obj)
+    if lacks:
+        sys.stderr.write(f"{TORCH_LIB.name} is left out: {lacks}\n")
+    else:
+        _link_torch_host(host.result())   # LIB is there whatever becomes of this
     return LIB
 
 

@@ -1,0 +1,42 @@
+"""The build without torch, in directories of the test's own."""
+import shutil
+from pathlib import Path
+
+import pytest
+
+from neural_block_textures_b200 import build as b
+
+
+@pytest.fixture
+def apart(tmp_path, monkeypatch):
+    """The build's outputs below tmp_path, made of one quick source."""
+    if not (shutil.which(b.nvcc()) or Path(b.nvcc()).exists()):
+        pytest.skip("no nvcc")
+    monkeypatch.setattr(b, "OUT_DIR", tmp_path / "lib")
+    monkeypatch.setattr(b, "BUILD_DIR", tmp_path / "obj")
+    monkeypatch.setattr(b, "LIB", tmp_path / "lib" / b.LIB.name)
+    monkeypatch.setattr(b, "TORCH_LIB", tmp_path / "lib" / b.TORCH_LIB.name)
+    monkeypatch.setattr(b, "SOURCES", ["ntcb_format.cpp"])
+    return tmp_path
+
+
+def test_without_torch_the_library_is_built(apart, monkeypatch, capsys):
+    monkeypatch.setattr(b.importlib.util, "find_spec", lambda name: None)
+    assert b.build() == b.LIB and b.LIB.exists() and not b.TORCH_LIB.exists()
+    assert "torch is not installed" in capsys.readouterr().err
+
+
+def test_without_python_headers_the_library_is_built(apart, monkeypatch, capsys):
+    monkeypatch.setattr(b.sysconfig, "get_paths", lambda: {"include": str(apart / "nowhere")})
+    assert b.build() == b.LIB and b.LIB.exists() and not b.TORCH_LIB.exists()
+    assert "headers" in capsys.readouterr().err
+
+
+def test_a_torch_that_does_not_compile_leaves_the_library(apart, monkeypatch):
+    """The failure is raised, after the library that does not need torch was linked."""
+    def failing():
+        raise RuntimeError("these headers do not fit")
+    monkeypatch.setattr(b, "_compile_torch_host", failing)
+    with pytest.raises(RuntimeError, match="do not fit"):
+        b.build()
+    assert b.LIB.exists()
