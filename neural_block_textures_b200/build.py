@@ -71,19 +71,26 @@ def _torch_host_lacks() -> str | None:
     return None
 
 
+def _torch_built_for(torch: Path) -> str:
+    """What the torch library's code depends on beside its sources: torch's C++ classes and the interpreter's ABI."""
+    return "\n".join([str(torch), (torch / "version.py").read_text(), sys.implementation.cache_tag, str(sysconfig.get_config_var("SOABI"))])
+
+
 def _compile_torch_host() -> Path:
     """torch_host.cpp against the installed torch's headers."""
     s = CSRC / TORCH_SOURCE
     obj = BUILD_DIR / (TORCH_SOURCE + ".o")
-    if not _stale(obj, _deps(s)):
-        return obj
+    stamp = BUILD_DIR / (TORCH_SOURCE + ".torch")   # the torch that the object is for
     torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    if not _stale(obj, _deps(s)) and stamp.exists() and stamp.read_text() == _torch_built_for(torch):
+        return obj
     cuda = Path(nvcc()).resolve().parent.parent
     inc = [torch / "include", torch / "include" / "torch" / "csrc" / "api" / "include", cuda / "include", sysconfig.get_paths()["include"]]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", *[f"-I{d}" for d in inc], "-c", str(s), "-o", str(obj)]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed for {TORCH_SOURCE}:\n{r.stdout}\n{r.stderr}")
+    stamp.write_text(_torch_built_for(torch))
     return obj
 
 

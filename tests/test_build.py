@@ -40,3 +40,27 @@ def test_a_torch_that_does_not_compile_leaves_the_library(apart, monkeypatch):
     with pytest.raises(RuntimeError, match="do not fit"):
         b.build()
     assert b.LIB.exists()
+
+
+def test_another_torch_is_compiled_for_again(apart, monkeypatch):
+    """The host side uses torch's C++ classes: an object of another torch, or of one that moved, does not stay."""
+    from types import SimpleNamespace
+    made = []
+
+    def compiler(cmd, **kw):
+        out = Path(cmd[cmd.index("-o") + 1])
+        made.append(out.name)
+        out.write_text("object")
+        return SimpleNamespace(returncode=0, stdout="", stderr="")
+
+    def torch(name, version):
+        where = apart / name
+        where.mkdir(exist_ok=True)
+        (where / "version.py").write_text(f"__version__ = '{version}'\n")
+        monkeypatch.setattr(b.importlib.util, "find_spec", lambda _: SimpleNamespace(submodule_search_locations=[str(where)]))
+        before = len(made)
+        b._compile_torch_host()
+        return len(made) - before
+    monkeypatch.setattr(b.subprocess, "run", compiler)
+    b.BUILD_DIR.mkdir()
+    assert [torch("a", "1.0"), torch("a", "1.0"), torch("a", "1.1"), torch("a", "1.1"), torch("b", "1.1"), torch("a", "1.1")] == [1, 0, 1, 0, 1, 1]
