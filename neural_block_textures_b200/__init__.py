@@ -13,8 +13,8 @@ from .trainer import Trainer
 __all__ = ["Trainer", "ModelDesc", "QesDesc", "DctDesc", "load_library", "ModelSpec", "LevelSpec", "TrainConfig",
            "CONFIGS", "config", "qat_grid_table"]
 
+# by name only: `import *` must not load torch
 _TORCH_NAMES = {"symbol_logprobs": "symbols", "symbol_logprobs_grad": "symbols", "SymbolLogprobs": "symbols", "AdamW": "optim"}
-__all__ += list(_TORCH_NAMES)
 
 
 def __getattr__(name):
@@ -23,3 +23,7 @@ def __getattr__(name):
         value = globals()[name] = getattr(import_module("." + _TORCH_NAMES[name], __name__), name)
         return value
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__():
+    return sorted({*globals(), *_TORCH_NAMES})

@@ -1,5 +1,7 @@
 """The build without torch, in directories of the test's own."""
 import shutil
+import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -64,3 +66,19 @@ def test_another_torch_is_compiled_for_again(apart, monkeypatch):
     monkeypatch.setattr(b.subprocess, "run", compiler)
     b.BUILD_DIR.mkdir()
     assert [torch("a", "1.0"), torch("a", "1.0"), torch("a", "1.1"), torch("a", "1.1"), torch("b", "1.1"), torch("a", "1.1")] == [1, 0, 1, 0, 1, 1]
+
+
+def test_star_import_does_without_torch():
+    """`import *` gives the names that need no torch and loads none; the operators come by name."""
+    code = ("import sys\n"
+            "sys.modules['torch'] = None\n"   # an import of it raises
+            "from neural_block_textures_b200 import *\n"
+            "assert callable(Trainer) and callable(config) and 'neural_block_textures_b200.symbols' not in sys.modules\n"
+            "import neural_block_textures_b200 as n\n"
+            "assert 'AdamW' in dir(n) and 'symbol_logprobs' in dir(n) and 'AdamW' not in globals()\n"
+            "try:\n"
+            "    n.AdamW\n"
+            "except ImportError:\n"
+            "    print('fine')\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=b.ROOT)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
