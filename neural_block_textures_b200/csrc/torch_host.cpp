@@ -6,6 +6,7 @@
 // exception must not leave an entry (it would end the process): torch throws them from as little as a size() of a tensor
 // subclass or a nested tensor, so everything is done inside torch's own translation to Python's exceptions.
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -68,6 +69,10 @@ PyObject* ntcb_host_logprobs(PyObject* logits, PyObject* symbols, int topk) {
         ntcb_symbol_desc d;
         if (!describe(logits, symbols, d) || topk < 0 || topk > NTCB_MAX_TOPK || topk > d.vocab) Py_RETURN_NONE;
         const at::Tensor x = THPVariable_Unpack(logits), s = THPVariable_Unpack(symbols);
+        if (((at::GradMode::is_enabled() && x.requires_grad()) || x._fw_grad(0).defined()) &&
+            PyErr_WarnEx(PyExc_UserWarning, "symbol_logprobs: the logits require a gradient, but autograd records nothing of this call: "
+                         "take it from symbol_logprobs_grad, and pass logits.detach() here", 2) < 0)   // 2: the caller's line
+            return nullptr;
         at::Tensor out[5];
         char why[256];
         bool ok;

@@ -2,11 +2,13 @@
 symbol (palette index, grid index, DCT token) under a row of logits, the row's entropy and its likeliest symbols, and
 the gradient of a rate loss for the logits. Where print_stats rates a level by its counts, this rates it by a model.
 
-    r = symbol_logprobs(logits, symbols, topk=4)          # logits [n, V] on the GPU, symbols [n]
+    r = symbol_logprobs(logits.detach(), symbols, topk=4)   # logits [n, V] on the GPU, symbols [n]
     bits = -r.logp / math.log(2)
     dlogits = symbol_logprobs_grad(logits, symbols, r.lse, r.entropy, dlogp=-1.0 / n)   # of the mean code length
 
-Calls run on torch's current stream of the logits' device, without synchronising; nothing is recorded by autograd.
+Calls run on torch's current stream of the logits' device, without synchronising. Nothing is recorded by autograd: logits
+that require a gradient are rated with a warning (pass logits.detach()), and symbol_logprobs_grad gives what to hand to
+their backward pass.
 """
 from __future__ import annotations
 

@@ -598,3 +598,29 @@ def test_cost_of_rows_far_from_zero(cuda_device):
             best = min(best, begin.elapsed_time(end))
         times.append(best)
     assert times[1] < 24 * times[0], times
+
+
+def test_logits_that_require_a_gradient(cuda_device):
+    """autograd records nothing, and says so: a warning on the caller's line, the same numbers."""
+    import warnings
+
+    import torch.autograd.forward_ad as forward_ad
+    x, s, _, _ = make(6, 9, "f32", masks=False)
+    want = symbol_logprobs(x, s, topk=2)
+    leaf = x.clone().requires_grad_()
+    with pytest.warns(UserWarning, match="records nothing") as seen:
+        got = symbol_logprobs(leaf, s, topk=2)
+    assert seen[0].filename == __file__ and not got.logp.requires_grad
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with forward_ad.dual_level(), pytest.warns(UserWarning, match="records nothing"):
+        symbol_logprobs(forward_ad.make_dual(x, torch.ones_like(x)), s)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        symbol_logprobs(leaf.detach(), s)
+        with torch.no_grad():
+            symbol_logprobs(leaf, s)
+        with pytest.raises(UserWarning):
+            symbol_logprobs(leaf, s)
+        d = symbol_logprobs_grad(leaf, s, want.lse, want.entropy, -1.0)   # the gradient itself, handed on
+    leaf.backward(d)
+    assert torch.equal(leaf.grad, d)
