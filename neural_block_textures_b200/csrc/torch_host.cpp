@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
+#include <vector>
 
 #include "../../include/ntc_b200.h"
 
@@ -53,6 +54,10 @@ struct Unlocked {
     PyThreadState* state = PyEval_SaveThread();
     ~Unlocked() { PyEval_RestoreThread(state); }
 };
+
+// Raises a tensor's version, as torch's own in-place operations do: a backward pass over values saved before then fails
+// instead of using the new ones. Inference tensors have no version.
+void written(const at::Tensor& t) { if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version(); }
 
 PyObject* failed(const char* name, const char* why) {
     PyErr_Format(PyExc_RuntimeError, "%s: %s", name, why);
@@ -122,11 +127,11 @@ PyObject* ntcb_host_logprobs_grad(PyObject* logits, PyObject* symbols, PyObject*
     END_HANDLE_TH_ERRORS
 }
 
-// The addresses of n parameters and gradients (lists; a gradient may be None: 0 for both) after checking sizes, types,
-// layout and device. Returns -1, or the index of the first tensor that does not fit (with the Python exception that it
-// raised, if it did), or -2 when the lists do not.
-int ntcb_host_addresses(PyObject* params, PyObject* grads, int n, const long long* sizes, const int* param_types, const int* grad_types,
-                        int device, uint64_t* pp, uint64_t* gg) {
+// A step of plan `a` over n parameters and gradients (lists; a gradient may be None) after checking sizes, types, layout and
+// device. Returns -1, or the index of the first tensor that does not fit (with the Python exception that it raised, if it
+// did), -2 when the lists do not, or -3 with a reason in why.
+int ntcb_host_adamw_step(const ntcb_adamw* a, PyObject* params, PyObject* grads, int n, const long long* sizes, const int* param_types,
+                         const int* grad_types, int device, void* state, const ntcb_adamw_args* args, char* why, size_t why_cap) {
     if (!PyList_Check(params) || !PyList_Check(grads) || PyList_GET_SIZE(params) != n || PyList_GET_SIZE(grads) != n) return -2;
     const auto fits = [&](PyObject* o, long long size, int type) {
         if (!plain(o)) return false;
@@ -135,19 +140,37 @@ int ntcb_host_addresses(PyObject* params, PyObject* grads, int n, const long lon
     };
     int i = 0;
     try {
+        std::vector<void*> at((size_t)n * 2, nullptr);
         for (; i < n; i++) {
             PyObject *p = PyList_GET_ITEM(params, i), *g = PyList_GET_ITEM(grads, i);
-            pp[i] = gg[i] = 0;
             if (g == Py_None) continue;
             if (!fits(p, sizes[i], param_types[i]) || !fits(g, sizes[i], grad_types[i])) return i;
-            pp[i] = reinterpret_cast<uint64_t>(THPVariable_Unpack(p).data_ptr());
-            gg[i] = reinterpret_cast<uint64_t>(THPVariable_Unpack(g).data_ptr());
+            at[i] = THPVariable_Unpack(p).data_ptr();
+            at[n + i] = THPVariable_Unpack(g).data_ptr();
         }
+        void* stream = stream_of(device);
+        bool ok;
+        {
+            const Unlocked unlocked;
+            ok = ntcb_adamw_step(a, at.data(), at.data() + n, state, args, stream, why, why_cap);
+        }
+        if (!ok) return -3;
+        for (int k = 0; k < n && k < PyList_GET_SIZE(params); k++)
+            if (at[n + k] && THPVariable_Check(PyList_GET_ITEM(params, k))) written(THPVariable_Unpack(PyList_GET_ITEM(params, k)));
+        return -1;
     } catch (python_error& e) {
         e.restore();
     } catch (...) {   // a tensor that does not say what it is, or has no memory
     }
-    return i < n ? i : -1;
+    return i;
+}
+
+// Raises the version of a tensor that a call wrote.
+PyObject* ntcb_host_written(PyObject* tensor) {
+    HANDLE_TH_ERRORS
+        if (THPVariable_Check(tensor)) written(THPVariable_Unpack(tensor));
+        Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
 }
 
 }  // extern "C"

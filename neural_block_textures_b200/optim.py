@@ -8,7 +8,8 @@ the Adam that runs inside the trainer's own steps. With weight_decay 0 it is tha
         opt.step(it, lr)
 
 A step runs on torch's current stream of the parameters' device, without synchronising, and writes the parameters in
-place (autograd does not see that write). In a captured CUDA graph the step number comes from the device: pass `it` as an
+place; autograd does not record that, but a backward pass over values saved before the step fails, as after torch's own
+in-place operations (a graph's replays are not seen). In a captured CUDA graph the step number comes from the device: pass `it` as an
 int64 tensor and advance it there. The graph has the addresses of the parameters, the gradients and the state: keep those
 tensors as long as it is replayed (the state stays by itself until close()).
 """
@@ -16,7 +17,6 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
-from array import array
 
 import torch
 
@@ -112,19 +112,19 @@ class AdamW:
         self._open()
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         n = len(self.params)
-        pp, gg = array("Q", bytes(8 * n)), array("Q", bytes(8 * n))
-        bad = _host.ntcb_host_addresses(self.params, grads, n, *self._plan, self._index, pp.buffer_info()[0], gg.buffer_info()[0])
-        if bad == -2:
-            raise ValueError(f"AdamW.step: {n} gradients are needed, not {len(grads)}")
-        if bad >= 0:
-            raise ValueError(f"AdamW.step: gradient {bad} must be a contiguous {self._grad_dtypes[bad]} tensor of {self._sizes[bad]} elements on "
-                             f"{self.device}, and its parameter as it was when the plan was made")
         it, it_dev = self._scalar(it, torch.int64, "it") if isinstance(it, _T) else (it, 0)
         lr, lr_dev = self._scalar(lr, torch.float32, "lr") if isinstance(lr, _T) else (lr, 0)
         grad_scale, scale_dev = self._scalar(grad_scale, torch.float32, "grad_scale") if isinstance(grad_scale, _T) else (grad_scale, 0)
         args = _pack_args(lr, *self.betas, self.eps, self.weight_decay, grad_scale, it, self.seed & 0xFFFFFFFFFFFFFFFF, it_dev, lr_dev, scale_dev)
-        _call(self.lib.ntcb_adamw_step, "AdamW.step", self.h, pp.buffer_info()[0], gg.buffer_info()[0], self.state.data_ptr(), args,
-              _raw_stream(self._index))
+        why = C.create_string_buffer(256)
+        bad = _host.ntcb_host_adamw_step(self.h, self.params, grads, n, *self._plan, self._index, self.state.data_ptr(), args, why, 256)
+        if bad == -2:
+            raise ValueError(f"AdamW.step: {n} gradients are needed, not {len(grads)}")
+        if bad == -3:
+            raise RuntimeError("AdamW.step: " + why.value.decode())
+        if bad >= 0:
+            raise ValueError(f"AdamW.step: gradient {bad} must be a contiguous {self._grad_dtypes[bad]} tensor of {self._sizes[bad]} elements on "
+                             f"{self.device}, and its parameter as it was when the plan was made")
 
     def moments_flat(self) -> tuple[torch.Tensor, torch.Tensor]:
         """(m, v) as flat float32 tensors, tensor i at offsets[i]: the state itself with 32 bits, the values that the

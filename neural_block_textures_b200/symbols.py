@@ -79,8 +79,9 @@ def _load_host() -> C.PyDLL:
     o = C.py_object
     lib.ntcb_host_logprobs.restype, lib.ntcb_host_logprobs.argtypes = o, [o, o, C.c_int]
     lib.ntcb_host_logprobs_grad.restype, lib.ntcb_host_logprobs_grad.argtypes = o, [o] * 6
-    lib.ntcb_host_addresses.restype = C.c_int
-    lib.ntcb_host_addresses.argtypes = [o, o, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]
+    p, i = C.c_void_p, C.c_int
+    lib.ntcb_host_adamw_step.restype, lib.ntcb_host_adamw_step.argtypes = i, [p, o, o, i, p, p, p, i, p, p, C.c_char_p, C.c_size_t]
+    lib.ntcb_host_written.restype, lib.ntcb_host_written.argtypes = o, [o]
     return lib
 
 
@@ -151,4 +152,5 @@ def symbol_logprobs_grad(logits: torch.Tensor, symbols: torch.Tensor, lse: torch
           lse.data_ptr(), entropy.data_ptr() if dentropy is not None else None, dlogp.data_ptr(), dlogp.stride(0),
           dentropy.data_ptr() if dentropy is not None else None, dentropy.stride(0) if dentropy is not None else 0, out.data_ptr(),
           out.stride(0) if n > 1 else v, _raw_stream(device))
+    _host.ntcb_host_written(out)
     return out

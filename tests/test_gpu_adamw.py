@@ -453,3 +453,25 @@ def test_device_scalars_off_their_alignment(cuda_device):
                                      C.addressof(args), None, why, 256)
         assert ok == 0 and b"aligned" in why.value
     assert (p == 1).all()
+
+
+def test_steps_are_seen_by_backward_passes(cuda_device):
+    """A step raises the version of the parameters that it wrote: values saved before it are not used with the new ones."""
+    p = [torch.nn.Parameter(torch.ones(40, device="cuda")), torch.nn.Parameter(torch.ones(5, device="cuda"))]
+    opt = AdamW(p)
+    before = [x._version for x in p]
+    loss = (p[0] * p[0]).sum()
+    opt.step(1, 0.1, [torch.ones(40, device="cuda"), None])
+    assert p[0]._version > before[0] and p[1]._version == before[1]
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    now = p[0]._version
+    with pytest.raises(RuntimeError):
+        opt.step(1, -0.1, [torch.ones(40, device="cuda"), None])   # refused: nothing was written
+    assert p[0]._version == now
+    (p[0] * p[0]).sum().backward()
+    assert torch.equal(p[0].grad, 2 * p[0].detach())
+    with torch.inference_mode():
+        q = torch.ones(6, device="cuda")
+    AdamW([q]).step(1, 0.1, [torch.ones(6, device="cuda")])   # has no version
+    assert (q < 1).all()

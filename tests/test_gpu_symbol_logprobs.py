@@ -624,3 +624,13 @@ def test_logits_that_require_a_gradient(cuda_device):
         d = symbol_logprobs_grad(leaf, s, want.lse, want.entropy, -1.0)   # the gradient itself, handed on
     leaf.backward(d)
     assert torch.equal(leaf.grad, d)
+
+
+def test_a_gradient_over_the_logits_is_seen_by_backward_passes(cuda_device):
+    x, s, _, _ = make(6, 9, "f32", masks=False)
+    r = symbol_logprobs(x, s)
+    w = torch.ones(6, 9, device="cuda", requires_grad=True)
+    loss = (w * x).sum()   # saves x
+    symbol_logprobs_grad(x, s, r.lse, r.entropy, -1.0, out=x)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
