@@ -100,7 +100,7 @@ def symbol_logprobs(logits: torch.Tensor, symbols: torch.Tensor, topk: int = 0) 
     if 0 <= topk <= abi.MAX_TOPK:
         r = _host.ntcb_host_logprobs(logits, symbols, topk)
         if r is not None:
-            return SymbolLogprobs(*r)
+            return tuple.__new__(SymbolLogprobs, r)   # the class's own __new__ takes its fields one by one: 0.3 us more
     _, n, v, _ = _desc(logits, symbols, "symbol_logprobs")   # says what is wrong
     if logits.is_neg():
         return symbol_logprobs(logits.resolve_neg(), symbols, topk)
