@@ -4,9 +4,12 @@
 //
 // Nothing is reduced over a tensor, so the step is bound by memory: 28 bytes per fp32 element with 32-bit moments (151 M
 // elements in 512 tensors: 610 us, 6.9 TB/s, above the rate of a plain copy), 16 with 8-bit ones (430 to 455 us, 5.3 to 5.6
-// TB/s: some 70 instructions an element keep the SMs issuing 70 % of the time; reading the moments as floats 230 us, 6.6
-// TB/s). Work is cut into chunks of one tensor; a CTA takes one chunk, found in a table that the plan keeps on the device,
-// and the tensors' addresses come with the launch (by value: they may change from step to step).
+// TB/s: some 75 instructions an element keep the SMs issuing 70 % of the time; the 48 registers that five CTAs an SM leave
+// cost 84 bytes of spills). With 16-bit tensors an 8-bit step moves 10 bytes an element but takes longer (13 M bf16 elements
+// 49 us, fp32 45; 151 M 624 and 484, all with the step number on the device): as many instructions, issued 55 % of the time
+// behind loads. Reading the moments as floats takes 230 us (6.6 TB/s). Work is cut into chunks of one tensor; a CTA takes one
+// chunk, found in a table that the plan keeps on the device, and the tensors' addresses come with the launch (by value: they
+// may change from step to step).
 //
 // 8-bit moments. Blocks of 256 elements, one warp each. A value is held as its float's exponent and upper 3 mantissa
 // bits, q = bits >> 20, counted from the base of the block's window, which ends at the block's largest q. The grid of q

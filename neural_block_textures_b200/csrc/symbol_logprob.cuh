@@ -8,6 +8,9 @@
 // bits whatever their type. Rows: no finite logit (everything masked) gives lse = logp = -inf, H = 0 and no alternatives;
 // a NaN or +inf gives NaN.
 //
+// Approximations, by choice: 2^y is the hardware's ex2.approx.ftz (2^-22 relative; results below 2^-126 are 0), and u / s and
+// a renormalised row's 1 / s are __fdividef (two units in the last place).
+//
 // Exponents (Scale below): e^d = 2^y with y = x L - mL in one fused multiply-add, L = log2 e and mL = m L rounded. All
 // y of a row are off by the same mL - m L, which is known exactly and put back where the row is finished, so the only
 // rounding is y's own. y is clamped at kYLow, where 2^y is 0 in 32 bits: -inf and the type's lowest value then add 0 to u,
@@ -528,8 +531,9 @@ __device__ __forceinline__ void rate_row(const RowArgs& a, const RowIn<T, E / VE
     }
 }
 
-// Measured: 2^18 x 256 bf16 29 us without alternatives (5.2 TB/s of the 6.5 that a copy reaches), 37 with one, 74 with eight
-// (the minima and maxima of the sorts, on the half-rate logic unit, near 80 % busy); 2^15 x 1024 fp32 at the memory's rate; 2^20 x 4
+// Measured: 2^18 x 256 bf16 29 us without alternatives (4.8 TB/s of the 6.5 that a copy reaches; the exponential and the logic
+// unit each some 55 % busy), 35 with one, 73 with eight (the minima and maxima of the sorts, on the half-rate logic unit, 79 %
+// busy), fp32 176 with eight (64-bit keys); 2^15 x 1024 fp32 at the memory's rate; 2^20 x 4
 // fp32 9.2 and, with two alternatives, 12.4 us (instruction issue: the row's end is paid by every lane).
 // One group of rows to a CTA. (CTAs that stay and fetch the next rows ahead were slower on short rows: 17 against 15 us for
 // 2^20 rows of 4; the hardware's turnover of CTAs hides more.)
@@ -581,8 +585,10 @@ __device__ __forceinline__ P peer_load(const P* p, unsigned rank) {   // a word 
 // by all threads together) and the few logits that reach it are sorted. Where many logits equal the bound (a row of one
 // value, a part masked by the lowest value) those above it are taken like this and the first equal ones in order; what
 // still is too much is gone through by one warp with a running list of 32.
-// Measured: 2048 x 65536 bf16 51 us (5.2 TB/s; the exponential unit alone needs 37), with 20 alternatives 62; 1024 x 65536
-// fp32 50 us (5.4 TB/s); 1 x 65536 fp32 on eight CTAs 5 us, with 20 alternatives 8 (latency).
+// Measured: 2048 x 65536 bf16 52 us (5.2 TB/s; the exponential unit alone needs 37), with 20 alternatives 62; 1024 x 65536
+// fp32 50 us (5.4 TB/s); 1 x 65536 fp32 on eight CTAs 5 us, with 20 alternatives 8 (latency). Many alternatives: 30000 x 4099
+// fp16 63 us without, 164 with 32; 2^25 bf16 logits in rows of 700 with 17 77 us, in rows of 1024 with 32 86 (the bound lets
+// too many logits through, and one warp of a row sorts them while the others wait).
 template <class T, class K, int W, int R>
 __global__ void __launch_bounds__(32 * W * R) k_logprobs_long(const RowArgs a, int C) {
     constexpr int N = VEC<T>, kThreads = 32 * W, U = 4;
