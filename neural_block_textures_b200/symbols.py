@@ -115,7 +115,7 @@ def symbol_logprobs_grad(logits: torch.Tensor, symbols: torch.Tensor, lse: torch
     """The gradient of sum(dlogp * logp + dentropy * entropy) for the logits, in their type, from the forward pass's lse
     and entropy. dlogp / dentropy: [n] float32 (any stride, so an expanded scalar too) or a number for every row.
     out: where to write it, of the logits' shape and type; the logits themselves are allowed, memory
-    that overlaps them otherwise is refused."""
+    that overlaps them otherwise is refused, and it must not overlap the other tensors."""
     if out is None and isinstance(dlogp, torch.Tensor) and (dentropy is None or isinstance(dentropy, torch.Tensor)):
         r = _host.ntcb_host_logprobs_grad(logits, symbols, lse, entropy, dlogp, dentropy)
         if r is not None:
@@ -125,10 +125,9 @@ def symbol_logprobs_grad(logits: torch.Tensor, symbols: torch.Tensor, lse: torch
     if out is not None and out.is_neg():
         raise ValueError("symbol_logprobs_grad: out must not be a negated view")
     # the memory of a negated view holds the values' negatives
-    given = [x.resolve_neg() if isinstance(x, torch.Tensor) else x for x in (logits, lse, entropy, dlogp, dentropy)]
-    if given[0] is not logits:
-        return symbol_logprobs_grad(given[0], symbols, *given[1:], out=out)
-    _, lse, entropy, dlogp, dentropy = given
+    if logits.is_neg():
+        return symbol_logprobs_grad(logits.resolve_neg(), symbols, lse, entropy, dlogp, dentropy, out)
+    lse, entropy, dlogp, dentropy = (x.resolve_neg() if isinstance(x, torch.Tensor) else x for x in (lse, entropy, dlogp, dentropy))
     if not isinstance(dlogp, torch.Tensor):
         dlogp = torch.full((1,), float(dlogp), device=dev).expand(n)
     if dentropy is not None and not isinstance(dentropy, torch.Tensor):

@@ -634,3 +634,15 @@ def test_a_gradient_over_the_logits_is_seen_by_backward_passes(cuda_device):
     symbol_logprobs_grad(x, s, r.lse, r.entropy, -1.0, out=x)
     with pytest.raises(RuntimeError, match="inplace"):
         loss.backward()
+
+
+def test_a_tensor_subclass_that_makes_new_objects(cuda_device):
+    class Fresh(torch.Tensor):
+        @classmethod
+        def __torch_function__(cls, func, types, args=(), kwargs=None):
+            r = super().__torch_function__(func, types, args, kwargs or {})
+            return r.detach().clone().as_subclass(cls) if func is torch.Tensor.resolve_neg else r
+    x, s, _, _ = make(6, 9, "f32", masks=False)
+    r = symbol_logprobs(x, s)
+    want = symbol_logprobs_grad(x, s, r.lse, r.entropy, -1.0, 0.5)
+    assert torch.equal(symbol_logprobs_grad(x.as_subclass(Fresh), s, r.lse, r.entropy.as_subclass(Fresh), -1.0, 0.5).as_subclass(torch.Tensor), want)
