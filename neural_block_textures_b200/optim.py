@@ -95,6 +95,9 @@ class AdamW:
         except Exception:
             pass
 
+    def __reduce_ex__(self, protocol):
+        raise TypeError("AdamW: a plan cannot be copied or pickled; use state_dict() and load_state_dict()")
+
     def _open(self) -> None:
         if not self.h:
             raise RuntimeError("AdamW: closed")

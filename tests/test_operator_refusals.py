@@ -217,3 +217,14 @@ def test_buffers_off_their_alignment():
     for bad in range(4):   # lse, entropy, dlogp, dentropy
         lse, entropy, dlogp, dentropy = [BUF + 2 * (i == bad) for i in range(4)]
         assert lib.ntcb_symbol_logprobs_grad(d, BUF, BUF, lse, entropy, dlogp, 1, dentropy, 1, BUF, 8, None, why, 256) == 0 and b"aligned" in why.value
+
+
+def test_an_optimiser_cannot_be_copied():
+    """A copy would free the plan of the original a second time."""
+    import copy
+    import pickle
+    opt = AdamW.__new__(AdamW)
+    opt.h = None
+    for make in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(TypeError, match="state_dict"):
+            make(opt)
